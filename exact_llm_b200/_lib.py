@@ -20,6 +20,13 @@ class Config(ctypes.Structure):
                                             "emb_shift")]
 
 
+class KvView(ctypes.Structure):
+    """exb_kv_view: a paged K/V cache (pointers, sizes, strides in elements)."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "ks", "v")]
+                + [(n, ctypes.c_int) for n in ("layers", "pages", "KV", "page", "hd")]
+                + [(f"{t}_{d}", ctypes.c_int64) for t in ("k", "s", "v") for d in ("layer", "page", "head", "pos")])
+
+
 # name -> (restype, argtypes); must list every entry point of include/exactb200.h
 SIGNATURES = {
     "exb_last_error": (ctypes.c_char_p, []),
@@ -36,6 +43,21 @@ SIGNATURES = {
     "exb_linear_channel": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "exb_tree_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 4),
+    "exb_tree_attention": (ctypes.c_int, [ctypes.POINTER(KvView), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
+                                          ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
+                                          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p,
+                                          ctypes.c_void_p]),
+    "exb_tree_verify": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                       ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
+                                       ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                       ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "exb_kv_compact": (ctypes.c_int, [ctypes.POINTER(KvView), ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
+                                      ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
+                                      ctypes.c_void_p, ctypes.c_void_p]),
+    "exb_kv_copy_pages": (ctypes.c_int, [ctypes.POINTER(KvView), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                         ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]),
     "exb_model_create": (ctypes.c_int, [ctypes.POINTER(Config), ctypes.POINTER(ctypes.c_void_p)]),
     "exb_model_destroy": (None, [ctypes.c_void_p]),
     "exb_model_set_tables": (ctypes.c_int, [ctypes.c_void_p, c_i64p, c_i64p, c_i64p, c_i64p, c_i64p]),

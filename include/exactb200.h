@@ -87,6 +87,70 @@ int exb_linear_g128_noalloc(const int64_t* x, int R, int K, const int8_t* w_NK, 
 int exb_linear_channel(const int64_t* x, int R, int K, const int8_t* w_NK, const int64_t* M, const int64_t* bias,
                        int N, int64_t* y, int64_t* acc_out, void* scratch, void* stream);
 
+/* ------------------------------------------- speculative decoding: trees of drafted tokens */
+
+/* A paged K/V cache as this engine stores rows: K int16 after RoPE and qrow with its shift (int8,
+ * 0..63), V int32 Q16.  Position p of a sequence lies in page table[seq][p / page] at offset
+ * p % page.  Strides are in elements; the hd values of a row are contiguous.  Alignment: k and v
+ * 16 bytes, the K strides multiples of 8 elements, the V strides multiples of 4.  A cache of one
+ * contiguous slot per sequence is the case page = its capacity, table[seq] = {slot}. */
+typedef struct exb_kv_view {
+  int16_t* k;
+  int8_t* ks;
+  int32_t* v;
+  int layers, pages, KV, page, hd;             /* hd 16, 32, 64 or 128 */
+  int64_t k_layer, k_page, k_head, k_pos;
+  int64_t s_layer, s_page, s_head, s_pos;
+  int64_t v_layer, v_page, v_head, v_pos;
+} exb_kv_view;
+
+/* The four calls below take device buffers, launch on `stream`, allocate nothing and do not
+ * synchronise.  `status` (device int32, may be NULL) gets bit 8 or-ed in when a kernel met an
+ * index outside its range (a page id, a position past the table, a malformed row range or path);
+ * such an entry is left out of the result, never read or written. */
+
+/* Exact attention of a tree of drafted tokens over the cache (the arithmetic of exact_llm.py:109-115,
+ * 164-176, experiments/speed_fair_kaggle.py:617-630; the tree mask has no counterpart there).
+ * Sequence b owns rows row_start[b] .. row_start[b+1]-1 of q (its tree, node i = row row_start[b]+i,
+ * cached at position ctx[b] + i).  A row sees the positions below ctx[b] and the nodes i whose bit
+ * i % 64 of mask[row][i / 64] is set; a row that sees nothing gives zeros.
+ *   q int16 (R, H, hd), qs int32 (R, H) shifts (0..63); layer 0 of kv is used; H % KV == 0
+ *   table int32 (B, max_pages), ctx int32 (B), row_start int32 (B+1), mask (R, mask_words)
+ *   exp_t int32 (10242) the Q24 table; out int64 (R, H, hd) */
+size_t exb_tree_attention_workspace_bytes(int R, int H, int KV, int hd);
+int exb_tree_attention(const exb_kv_view* kv, const int16_t* q, const int32_t* qs, int R, int H, const int32_t* table,
+                       int B, int max_pages, const int32_t* ctx, const int32_t* row_start, const uint64_t* mask,
+                       int mask_words, const int32_t* exp_t, int64_t* out, void* workspace, size_t workspace_bytes,
+                       int32_t* status, void* stream);
+
+/* Verification of drafted trees against the target's own choice (exact_llm.py:243-259).  Row r's
+ * logits (int64, row stride ld) give sampled[r]: the first index whose running sum of the Q20
+ * probabilities of shr(logit * tnum, 16) exceeds (u20[r] * total) >> 20, or, where u20[r] < 0, the
+ * lowest index of the largest logit.  Then, for every sequence, the walk from node 0: at node c the
+ * target's token is sampled[c]; the lowest node whose parent is c and whose token equals it is
+ * accepted and the walk goes on there, otherwise it ends.
+ *   tokens, parent int32 (R): the drafted token of every row and its parent's index in the sequence
+ *     (a row never follows one that is not before it: parent < own index; -1 for node 0)
+ *   path, out_tokens int32 (B, max_len): the accepted nodes (node 0 first) and the target's token at
+ *     each, -1 past the end; n int32 (B): their number, at most max_len.  The last token is new. */
+int exb_tree_verify(const int64_t* logits, int64_t ld, int R, int V, const int32_t* u20, int64_t tnum,
+                    const int32_t* tokens, const int32_t* parent, const int32_t* row_start, int B, int max_len,
+                    const int32_t* exp_t, int32_t* sampled, int32_t* n, int32_t* path, int32_t* out_tokens,
+                    void* stream);
+
+/* Keep the accepted path of every sequence: row ctx[b] + path[b][j] moves to ctx[b] + j for j < n[b],
+ * in every layer (path strictly increasing, as exb_tree_verify gives it; ld_path its row stride), and
+ * new_ctx[b] = ctx[b] + n[b].  A malformed path leaves its sequence as it was (new_ctx[b] = ctx[b]).
+ * The pages written must belong to one sequence only. */
+int exb_kv_compact(const exb_kv_view* kv, const int32_t* table, int B, int max_pages, const int32_t* ctx,
+                   const int32_t* path, int ld_path, const int32_t* n, int32_t* new_ctx, int32_t* status, void* stream);
+
+/* Copy the first rows[i] positions of page src[i] to page dst[i] in every layer, i < count (a forked
+ * sequence's last page, a shared page about to be written, a slot's prefix).  No page may be the
+ * target of two copies, nor source and target of different ones. */
+int exb_kv_copy_pages(const exb_kv_view* kv, const int32_t* src, const int32_t* dst, const int32_t* rows, int count,
+                      int32_t* status, void* stream);
+
 /* --------------------------------------------------------------------- model level */
 
 int exb_model_create(const exb_config* cfg, exb_model** out);
