@@ -5,13 +5,421 @@
 //
 // p needs the row's final maximum and sum (a floor division by the sum: no rescaling afterwards
 // gives the same bits), so a row goes over its positions three times.
+#include <cooperative_groups.h>
+
+#include <algorithm>
 #include <cmath>
 
 #include "exb_internal.h"
 #include "treedev.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace exb {
 
+// ---------------------------------------------------------------- few rows: one cluster per row tile
+// A cluster of CTAs takes one (sequence, KV head) and NR = 8 NT of its query rows (a group's heads of
+// neighbouring nodes together, so each K/V byte is read once for all of them); its CTAs split the
+// positions.  Scores are int8 tensor-core products over byte digits, x = 256 hi + lo (hi signed, lo
+// not): q.k = 65536 hh + 256 (hl + lh) + ll, each digit sum over 128 dims below 2^31.  They stay in
+// shared memory as 32-bit numbers (rows above 2^31: as distances from the CTA's own maximum) while
+// the cluster exchanges maxima and sums, so K and V are read once.  p < 2^21 is three byte digits,
+// V four: twelve digit products, the ones of equal weight 2^(8 s) summed in int32 (at most 3 * 2^16 per
+// position and 8192 positions a CTA) and put together in 64 bits at the end.
+constexpr int TC_THREADS_T = 256;
+constexpr int TREE_SMEM_MAX = 220 * 1024;
+constexpr int EXP_BULK = 40960;                    // bytes of the table that one bulk copy brings
+
+template <int HD, int NT>
+struct TreeGeo {
+  static constexpr int NR = 8 * NT;
+  static constexpr int DG = HD < 32 ? 1 : HD / 32;           // 32-dim groups of the output
+  static constexpr int KP = 8 / DG;                          // warps that share a dim group: key parts
+  static constexpr int KS = HD < 32 ? 1 : HD / 32;           // 32-dim steps of a score
+  static constexpr int OUT = KP * NR * HD;                   // partial outputs (int64)
+  static size_t smem(int ldk) { return 41024 + (size_t)OUT * 8 + (size_t)NR * ldk * 4; }
+};
+// score row pitch for n positions: 4 mod 16 words, so a warp's stores and loads hit 32 banks
+inline int tree_pitch(int64_t n) { return (int)((n + 15) / 16 * 16 + 4); }
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(const TreeArgs a, int ldk) {
+  using G = TreeGeo<HD, NT>;
+  constexpr int NR = G::NR;
+  extern __shared__ __align__(128) unsigned char sm[];
+  int32_t* T = reinterpret_cast<int32_t*>(sm);                               // exp table
+  int64_t* pout = reinterpret_cast<int64_t*>(sm + 41024);                    // KP x NR x HD
+  int32_t* sc = reinterpret_cast<int32_t*>(sm + 41024 + (size_t)G::OUT * 8); // NR x ldk
+  __shared__ int64_t lmax[NR], lsum[NR];
+  __shared__ int64_t wmax[8][NR];
+  __shared__ uint64_t pinv[NR], psum[NR];
+  __shared__ int32_t base[NR];
+  __shared__ int qsh[NR];
+  __shared__ const uint64_t* rmask[NR];
+  __shared__ int find[2];
+  __shared__ int odd_sh;
+  __shared__ uint64_t tbar;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), c = (int)cluster.block_rank();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
+  const int j = blockIdx.y, ct = (int)blockIdx.x / C;
+  const exb_kv_view& kv = a.kv;
+
+  // ---- this cluster's sequence and row tile: tiles of all sequences in order
+  if (warp == 0) {
+    int at = 0, fb = -1, ft = 0;
+    bool odd = lane == 0 && (a.B == 0 || a.row_start[0] != 0 || a.row_start[a.B] != a.R);
+    for (int b0 = 0; b0 < a.B && (fb < 0 || blockIdx.x == 0); b0 += 32) {
+      const int b = b0 + lane;
+      TreeSeq s;
+      if (b < a.B) {
+        s = tree_seq(a, b, blockIdx.x == 0 && j == 0);
+        odd |= s.T != a.row_start[b + 1] - a.row_start[b];
+      }
+      const int nt = (s.T * a.rep + NR - 1) / NR;
+      int inc = nt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const int w = __shfl_up_sync(0xffffffffu, inc, o); inc += lane >= o ? w : 0; }
+      const unsigned hit = __ballot_sync(0xffffffffu, ct < at + inc && ct >= at + inc - nt);
+      if (hit && fb < 0) {
+        const int l = __ffs(hit) - 1;
+        fb = b0 + l;
+        ft = ct - at - __shfl_sync(0xffffffffu, inc - nt, l);
+      }
+      at += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    odd = __any_sync(0xffffffffu, odd);
+    if (lane == 0) { find[0] = fb; find[1] = ft; odd_sh = odd; }
+    if (lane == 0) {
+      mbar_init(&tbar, 1);
+      mbar_fence_init();
+    }
+  }
+  __syncthreads();
+  // rows that no sequence owns: zeros, from the first CTA of every KV head
+  if (blockIdx.x == 0 && odd_sh) {
+    for (int r = warp; r < a.R; r += 8) {
+      bool own = false;
+      for (int b = lane; b < a.B; b += 32) {
+        const TreeSeq s = tree_seq(a, b, false);
+        own |= r >= s.r0 && r < s.r0 + s.T;
+      }
+      if (!__any_sync(0xffffffffu, own))
+        for (int e = lane; e < a.rep * HD; e += 32) a.out[((size_t)r * a.H + j * a.rep) * HD + e] = 0;
+    }
+  }
+  const int b = find[0];
+  if (b < 0) return;                                         // the whole cluster leaves together
+  const TreeSeq sq = tree_seq(a, b, false);
+  if (tid == 0) {                                            // the table arrives during the scores
+    mbar_expect_tx(&tbar, EXP_BULK);
+    bulk_g2s(T, a.exp_t, EXP_BULK, &tbar);
+  }
+  if (tid < EXP_LEN - EXP_BULK / 4) T[EXP_BULK / 4 + tid] = a.exp_t[EXP_BULK / 4 + tid];
+  const int32_t* trow = a.table + (size_t)b * a.MP;
+  const int g0 = find[1] * NR, ng = min(NR, sq.T * a.rep - g0);
+  // row i of the tile: node (g0 + i) / rep, head (g0 + i) % rep of the group
+  auto q_index = [&](int i) {
+    const int node = (g0 + i) / a.rep;
+    return (size_t)(sq.r0 + node) * a.H + (size_t)j * a.rep + (g0 + i - node * a.rep);
+  };
+  if (tid < NR) {
+    const bool live = tid < ng;
+    qsh[tid] = live ? a.qs[q_index(tid)] : 0;
+    rmask[tid] = a.mask + (size_t)(live ? sq.r0 + (g0 + tid) / a.rep : 0) * a.W;
+  }
+  // positions of this CTA, a multiple of 16 apart
+  const int chunk = ((sq.S + C - 1) / C + 15) & ~15;
+  const int t0 = min(sq.S, c * chunk), n = min(sq.S, t0 + chunk) - t0;
+  const int n32 = (n + 31) & ~31;
+
+  // ---- query digits: operand B of the scores; contraction slots 4 tq + i and 16 + 4 tq + i of a step
+  // hold dims 8 tq + i and 8 tq + 4 + i, so that a key row is read 16 bytes at a time
+  uint32_t ql[NT][G::KS][2], qh[NT][G::KS][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int i = nt * 8 + g;
+#pragma unroll
+    for (int ks = 0; ks < G::KS; ++ks) {
+      int4 v = make_int4(0, 0, 0, 0);
+      if (i < ng && ks * 32 + 8 * tq < HD)
+        v = *reinterpret_cast<const int4*>(a.q + q_index(i) * HD + ks * 32 + 8 * tq);
+      uint2 lo, hi;
+      int16_digits(v, lo, hi);
+      ql[nt][ks][0] = lo.x; ql[nt][ks][1] = lo.y;
+      qh[nt][ks][0] = hi.x; qh[nt][ks][1] = hi.y;
+    }
+  }
+  __syncthreads();
+  int qmax = 0;
+  bool qneg = false;
+#pragma unroll
+  for (int i = 0; i < NR; ++i) { qmax = max(qmax, qsh[i]); qneg |= qsh[i] < 0; }
+  int qs_r[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int f = 0; f < 2; ++f) qs_r[nt][f] = qsh[nt * 8 + 2 * tq + f];
+
+  // ---- phase 1: scores of 16 positions a warp and step (operand A: keys g and g + 8), 64-bit maxima.
+  // 19 <= 32 - qs - ks <= 32 for every row and key: |score| < 2^31 and a 32-bit shift gives it.
+  // Where some shift is outside, the CTA goes over its keys twice: maxima, then clamped distances.
+  const int c2 = (int)(a.inv << 16), c1 = (int)(a.inv << 8), c0 = (int)a.inv;
+  int64_t mx[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = INT64_MIN;
+  // one sweep over the keys: `wide` scores in 64 bits, `store` into sc
+  auto sweep = [&](auto wide_t, bool store, bool track) {
+    constexpr bool wide = decltype(wide_t)::value;
+    bool fits = true;
+    for (int u = warp * 16; u < n; u += 128) {
+      int sh[2], pgs[2];
+      const int16_t* kr[2];
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        const int t = u + g + 8 * f;
+        int off = 0;
+        pgs[f] = t < n ? page_of(a, trow, t0 + t, off) : -1;
+        kr[f] = k_row(kv, j, max(pgs[f], 0), off);
+        sh[f] = pgs[f] >= 0 ? k_shift(kv, j, pgs[f], off) : 0;
+        if (store && pgs[f] >= 0 && tq == 0)                 // V is needed after the exchanges: into L2 now
+          prefetch_l2_bulk(v_row(kv, j, pgs[f], off), HD * 4);
+      }
+      if (!wide) fits &= sh[0] + qmax <= 13 && sh[1] + qmax <= 13 && sh[0] >= 0 && sh[1] >= 0;
+      int4 kk[2][G::KS];
+#pragma unroll
+      for (int f = 0; f < 2; ++f)
+#pragma unroll
+        for (int ks = 0; ks < G::KS; ++ks)
+          kk[f][ks] = pgs[f] >= 0 && ks * 32 + 8 * tq < HD ? *reinterpret_cast<const int4*>(kr[f] + ks * 32 + 8 * tq)
+                                                            : make_int4(0, 0, 0, 0);
+      int ll[NT][4], md[NT][4], hh[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) ll[nt][f] = md[nt][f] = hh[nt][f] = 0;
+#pragma unroll
+      for (int ks = 0; ks < G::KS; ++ks) {
+        uint2 l0, h0, l1, h1;
+        int16_digits(kk[0][ks], l0, h0);
+        int16_digits(kk[1][ks], l1, h1);
+        const uint32_t al[4] = {l0.x, l1.x, l0.y, l1.y}, ah[4] = {h0.x, h1.x, h0.y, h1.y};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma_digits<false, false>(ll[nt], al, ql[nt][ks][0], ql[nt][ks][1]);
+          mma_digits<false, true>(md[nt], al, qh[nt][ks][0], qh[nt][ks][1]);
+          mma_digits<true, false>(md[nt], ah, ql[nt][ks][0], ql[nt][ks][1]);
+          mma_digits<true, true>(hh[nt], ah, qh[nt][ks][0], qh[nt][ks][1]);
+        }
+      }
+      const bool tree = t0 + u + 15 >= sq.ctx;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          const int kf = f >> 1, i = nt * 8 + 2 * tq + (f & 1), t = u + g + 8 * kf;
+          bool see = pgs[kf] >= 0;
+          if (tree && see && t0 + t >= sq.ctx) {
+            const int node = t0 + t - sq.ctx;
+            see = (rmask[i][node >> 6] >> (node & 63)) & 1;
+          }
+          const int sft = 32 - qs_r[nt][f & 1] - sh[kf];
+          if (!wide) {
+            const int64_t x = mad_wide_s32(hh[nt][f], c2, mad_wide_s32(md[nt][f], c1, mad_wide_s32(ll[nt][f], c0,
+                                                                        (int64_t)(1ull << ((sft - 1) & 63)))));
+            const int s = shift_low(x, sft);
+            if (see && s > mx[nt][f & 1]) mx[nt][f & 1] = s;
+            sc[i * ldk + t] = see ? s : INT32_MIN;
+          } else {
+            const int64_t acc = mad_wide_s32(hh[nt][f], 65536, mad_wide_s32(md[nt][f], 256, (int64_t)ll[nt][f]));
+            const int64_t s = shr64((int64_t)((uint64_t)acc * (uint64_t)a.inv), sft);
+            if (track && see && s > mx[nt][f & 1]) mx[nt][f & 1] = s;
+            if (store) {                                     // s - the CTA's maximum, clamped
+              const uint64_t d = see ? (uint64_t)lmax[i] - (uint64_t)s : ~0ull;
+              sc[i * ldk + t] = d < (1ull << 30) ? -(int)d : INT32_MIN;
+            }
+          }
+        }
+    }
+    return fits;
+  };
+  // row maxima of the CTA: lanes of a row (stride 4), then the warps
+  auto cta_max = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        int64_t m = mx[nt][f];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) { const int64_t w = __shfl_xor_sync(0xffffffffu, m, o); m = w > m ? w : m; }
+        if (g == 0) wmax[warp][nt * 8 + 2 * tq + f] = m;
+      }
+    __syncthreads();
+    if (tid < NR) {
+      int64_t m = wmax[0][tid];
+#pragma unroll
+      for (int w = 1; w < 8; ++w) m = wmax[w][tid] > m ? wmax[w][tid] : m;
+      lmax[tid] = m;
+    }
+    __syncthreads();
+  };
+  const bool fits = sweep(std::false_type{}, true, true);
+  const bool wide = __syncthreads_or(!fits || qneg);
+  if (wide) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = INT64_MIN;
+    sweep(std::true_type{}, false, true);
+    cta_max();
+    sweep(std::true_type{}, true, false);
+  } else {
+    cta_max();
+  }
+  // hidden rows of the tail, so that the loops below take whole steps of 32
+  for (int e = tid; e < NR * (n32 - n); e += TC_THREADS_T) {
+    const int i = e / (n32 - n);
+    sc[i * ldk + n + e - i * (n32 - n)] = INT32_MIN;
+  }
+  cluster.sync();
+  if (tid < NR) {
+    int64_t m = INT64_MIN;
+    for (int cc = 0; cc < C; ++cc) { const int64_t w = cluster.map_shared_rank(lmax, cc)[tid]; m = w > m ? w : m; }
+    // distance of a stored score: base - sc as 32 bits without a sign
+    if (wide) {
+      const uint64_t d = (uint64_t)m - (uint64_t)lmax[tid];
+      base[tid] = d < (1ull << 30) ? (int)d : (1 << 30);
+    } else {
+      base[tid] = m > INT32_MAX ? INT32_MAX : (int)m;        // another CTA's row may be far above
+    }
+  }
+  if (!mbar_wait(&tbar, 0)) set_err(a.status, ERR_WAIT_TIMEOUT);             // the table
+  __syncthreads();
+  // ---- phase 2: e over the stored scores, row sums
+#pragma unroll 1
+  for (int i = warp; i < NR; i += 8) {
+    int64_t s = 0;
+    const int bs = base[i];
+    for (int t = lane; t < n32; t += 32) {
+      const int v = sc[i * ldk + t];
+      const uint32_t e = v == INT32_MIN ? 0u : exp_sm(T, (uint32_t)bs - (uint32_t)v);
+      sc[i * ldk + t] = (int)e;
+      s += e;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) lsum[i] = s;
+  }
+  cluster.sync();
+  if (tid < NR) {
+    uint64_t s = 0;
+    for (int cc = 0; cc < C; ++cc) s += (uint64_t)cluster.map_shared_rank(lsum, cc)[tid];
+    psum[tid] = s;
+    pinv[tid] = prob_inverse(s);
+  }
+  __syncthreads();
+  // ---- phase 3: out += p . v.  Warp: 32 dims (its group) x every KP-th step of 32 positions.  Operand
+  // A: V digits, tile pair rows (tile 0: g, g + 8; tile 1: g, g + 8) = dims 4 g .. 4 g + 3, contraction
+  // slots 4 tq + i, 16 + 4 tq + i = positions tq + 4 i, tq + 16 + 4 i; operand B: p digits, row g.
+  {
+    const int dg = warp % G::DG, part = warp / G::DG;
+    const bool dlive = HD >= 32 || g < 4;
+    int acc[NT][2][6][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int w = 0; w < 6; ++w)
+#pragma unroll
+          for (int f = 0; f < 4; ++f) acc[nt][mt][w][f] = 0;
+    uint64_t inv[NT], sum[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) { inv[nt] = pinv[nt * 8 + g]; sum[nt] = psum[nt * 8 + g]; }
+    auto load_v = [&](int u, int4* v) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int t = u + tq + 4 * i;
+        int off = 0;
+        const int pg = t < n ? page_of(a, trow, t0 + t, off) : -1;
+        v[i] = pg >= 0 && dlive ? __ldg(reinterpret_cast<const int4*>(v_row(kv, j, pg, off) + dg * 32 + 4 * g))
+                                : make_int4(0, 0, 0, 0);
+      }
+    };
+    int4 v[8];
+    if (part * 32 < n) load_v(part * 32, v);
+#pragma unroll 1
+    for (int u = part * 32; u < n; u += 32 * G::KP) {
+      uint32_t va[2][4][4];                                  // tile, digit, fragment
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t* x = reinterpret_cast<const uint32_t*>(&v[4 * h]);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          uint32_t o[4];
+          byte_planes(x[d], x[4 + d], x[8 + d], x[12 + d], o);
+#pragma unroll
+          for (int p = 0; p < 4; ++p) va[d >> 1][p][(d & 1) + 2 * h] = o[p];
+        }
+      }
+      if (u + 32 * G::KP < n) load_v(u + 32 * G::KP, v);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        uint32_t pb[2][4];                                   // half, digit
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t p[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t e = (uint32_t)sc[(nt * 8 + g) * ldk + u + tq + 16 * h + 4 * i];
+            p[i] = inv[nt] ? prob_of(e, inv[nt]) : prob_slow(e, sum[nt]);
+          }
+          byte_planes(p[0], p[1], p[2], p[3], pb[h]);
+        }
+#pragma unroll
+        for (int pd = 0; pd < 3; ++pd)
+#pragma unroll
+          for (int vd = 0; vd < 4; ++vd)
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+              if (vd == 3) mma_digits<true, false>(acc[nt][mt][pd + vd], va[mt][vd], pb[0][pd], pb[1][pd]);
+              else mma_digits<false, false>(acc[nt][mt][pd + vd], va[mt][vd], pb[0][pd], pb[1][pd]);
+            }
+      }
+    }
+    // the weights put together; fragment f: dim 4 g + 2 mt + (f >> 1), row 2 tq + (f & 1)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          uint64_t s = 0;
+#pragma unroll
+          for (int w = 0; w < 6; ++w) s += (uint64_t)(int64_t)acc[nt][mt][w][f] << (8 * w);
+          if (dlive) pout[(size_t)(part * NR + nt * 8 + 2 * tq + (f & 1)) * HD + dg * 32 + 4 * g + 2 * mt + (f >> 1)] = (int64_t)s;
+        }
+  }
+  __syncthreads();
+  if (G::KP > 1) {
+    for (int e = tid; e < NR * HD; e += TC_THREADS_T) {
+      int64_t s = pout[e];
+#pragma unroll
+      for (int k = 1; k < G::KP; ++k) s += pout[k * NR * HD + e];
+      pout[e] = s;
+    }
+  }
+  cluster.sync();
+  // ---- the cluster's partial sums: CTA c finishes a slice of the rows
+  const int tot = ng * HD, per = (tot + C - 1) / C;
+  for (int e = c * per + tid; e < min(tot, (c + 1) * per); e += TC_THREADS_T) {
+    int64_t s = 0;
+    for (int cc = 0; cc < C; ++cc) s += cluster.map_shared_rank(pout, cc)[e];
+    const int i = e / HD;
+    a.out[q_index(i) * HD + (e - i * HD)] = shr64(s, 20);
+  }
+  cluster.sync();                                            // peers' shared memory stays until it is read
+}
+
+// ---------------------------------------------------------------- any size, slowly
 // One CTA per (row, head): the scores are computed anew in each of the three passes.
 constexpr int TS_THREADS = 128;
 
@@ -40,7 +448,7 @@ __global__ void __launch_bounds__(TS_THREADS) k_tree_simple(const TreeArgs a) {
   // score of position t; false where it is hidden
   auto score = [&](int t, int64_t& s, int& pg, int& off) {
     if (t >= sq.S || !seen(t)) return false;
-    pg = page_of(kv, row, t, off, a.status);
+    pg = page_of(a, row, t, off);
     if (pg < 0) return false;
     const int16_t* k = kv.k + (int64_t)pg * kv.k_page + (int64_t)j * kv.k_head + (int64_t)off * kv.k_pos;
     int64_t acc = 0;
@@ -91,7 +499,56 @@ __global__ void __launch_bounds__(TS_THREADS) k_tree_simple(const TreeArgs a) {
   if (tid < hd) out[tid] = shr64((int64_t)acc, 20);
 }
 
+template <int HD, int NT>
+static cudaError_t launch_cluster(const TreeArgs& a, int C, int ldk, cudaStream_t st) {
+  using G = TreeGeo<HD, NT>;
+  static DevOnce attr_set;
+  if (!attr_set.done()) {
+    cudaError_t e = cudaFuncSetAttribute(k_tree_cluster<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, TREE_SMEM_MAX);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_tree_cluster<HD, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    attr_set.set();
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)C * (unsigned)((int64_t)a.R * a.rep / G::NR + a.B), a.kv.KV);
+  cfg.blockDim = dim3(TC_THREADS_T);
+  cfg.dynamicSmemBytes = G::smem(ldk);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)C;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_tree_cluster<HD, NT>, a, ldk);
+}
+
+template <int NT>
+static cudaError_t launch_cluster_hd(const TreeArgs& a, int C, int ldk, cudaStream_t st) {
+  switch (a.kv.hd) {
+    case 16: return launch_cluster<16, NT>(a, C, ldk, st);
+    case 32: return launch_cluster<32, NT>(a, C, ldk, st);
+    case 64: return launch_cluster<64, NT>(a, C, ldk, st);
+    default: return launch_cluster<128, NT>(a, C, ldk, st);
+  }
+}
+
 static cudaError_t launch_tree_attention(const TreeArgs& a, cudaStream_t st) {
+  // rows per tile: 16 where the trees have that many in a group
+  const int NT = (int64_t)a.R * a.rep > 8ll * a.B ? 2 : 1, NR = 8 * NT;
+  // CTAs per cluster: as many as keep every cluster resident at once (two CTAs an SM, one with 16 rows
+  // or a long score array), each with 64 positions at least; more where the scores need the room
+  const int64_t clusters = std::max<int64_t>(a.B, ((int64_t)a.R * a.rep + NR - 1) / NR) * a.kv.KV;
+  auto pitch = [&](int c) { return tree_pitch(((a.cap + c - 1) / c + 31) / 16 * 16); };
+  auto smem_of = [&](int c) { return 41024 + (size_t)2048 * NR + (size_t)NR * pitch(c) * 4; };
+  int C = 1;
+  while (C < 16 && (smem_of(C) > (size_t)TREE_SMEM_MAX ||
+                    ((int64_t)C * 64 < a.cap && clusters * 2 * C <= (NT == 2 || smem_of(2 * C) > 110 * 1024 ? 148 : 296))))
+    C *= 2;
+  const size_t smem = smem_of(C);
+  const int ldk = pitch(C);
+  if (smem <= (size_t)TREE_SMEM_MAX)
+    return NT == 2 ? launch_cluster_hd<2>(a, C, ldk, st) : launch_cluster_hd<1>(a, C, ldk, st);
   k_tree_simple<<<dim3(a.R, a.H), TS_THREADS, 0, st>>>(a);
   return cudaGetLastError();
 }
@@ -136,15 +593,16 @@ int exb_tree_attention(const exb_kv_view* kv, const int16_t* q, const int32_t* q
     TREE_FAIL(EXB_EINVAL, "exb_tree_attention: null argument");
   if (mask_words < 1 || mask_words > 64 || max_pages < 1) TREE_FAIL(EXB_EINVAL, "exb_tree_attention: 1 <= mask_words <= 64 and max_pages >= 1");
   if ((int64_t)max_pages * kv->page >= (1ll << 30)) TREE_FAIL(EXB_EINVAL, "exb_tree_attention: a table row names 2^30 positions or more");
-  if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) TREE_FAIL(EXB_EINVAL, "exb_tree_attention: q, out and workspace must be 16-byte aligned");
+  if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)exp_t | (uintptr_t)workspace) & 15) TREE_FAIL(EXB_EINVAL, "exb_tree_attention: q, exp_t, out and workspace must be 16-byte aligned");
   if (!workspace || workspace_bytes < exb_tree_attention_workspace_bytes(R, H, kv->KV, kv->hd))
     TREE_FAIL(EXB_EINVAL, "exb_tree_attention: workspace too small");
   TreeArgs a;
   a.kv = *kv; a.q = q; a.qs = qs; a.table = table; a.ctx = ctx; a.row_start = row_start; a.mask = mask;
   a.exp_t = exp_t; a.out = out; a.status = status; a.R = R; a.H = H; a.rep = H / kv->KV; a.B = B; a.MP = max_pages;
-  a.W = mask_words; a.cap = (int64_t)max_pages * kv->page;
+  a.W = mask_words; a.cap = (int64_t)max_pages * kv->page; a.page_div = fast_div(kv->page);
   a.inv = (int64_t)std::nearbyint(65536.0 / std::sqrt((double)kv->hd));
-  const cudaError_t e = launch_tree_attention(a, (cudaStream_t)stream);
+  const cudaError_t e = B ? launch_tree_attention(a, (cudaStream_t)stream)
+                          : cudaMemsetAsync(out, 0, (size_t)R * H * kv->hd * 8, (cudaStream_t)stream);
   if (e != cudaSuccess) TREE_FAIL(EXB_ECUDA, std::string("exb_tree_attention: ") + cudaGetErrorString(e));
   return EXB_OK;
 }

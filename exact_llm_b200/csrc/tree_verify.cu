@@ -3,12 +3,14 @@
 //
 //   y = shr(logit * tnum, 16), p = (e << 20) // sum(e) with e the exp table at (max y - y),
 //   token = first index whose running sum of p exceeds (u20 * sum(p)) >> 20     (exact_llm.py:243-259)
+#include <cooperative_groups.h>
+
 #include "exb_internal.h"
 #include "treedev.cuh"
 
-namespace exb {
+namespace cg = cooperative_groups;
 
-constexpr int TV_THREADS = 1024;
+namespace exb {
 
 struct VerArgs {
   const int64_t* logits = nullptr; int64_t ld = 0;
@@ -19,25 +21,19 @@ struct VerArgs {
   int R = 0, V = 0, B = 0, max_len = 0;
 };
 
-// One CTA per row; thread t owns the t-th of 1024 contiguous slices of the row.
-__global__ void __launch_bounds__(TV_THREADS) k_tree_sample(const VerArgs a) {
-  __shared__ uint64_t red[TV_THREADS / 32];
-  __shared__ int64_t scan[TV_THREADS];
+// A row by one CTA of NT threads that reads it again for every step: any length, any values.
+// Thread t owns the t-th of NT contiguous slices of the row.
+template <int NT>
+EXB_DEV void sample_row(const VerArgs& a, int r) {
+  __shared__ uint64_t red[NT / 32];
+  __shared__ int64_t scan[NT];
   __shared__ int tok;
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t* row = a.logits + (int64_t)r * a.ld;
   const int u = a.u20[r];
-  const int c0 = (int)((int64_t)a.V * tid / TV_THREADS), c1 = (int)((int64_t)a.V * (tid + 1) / TV_THREADS);
+  const int c0 = (int)((int64_t)a.V * tid / NT), c1 = (int)((int64_t)a.V * (tid + 1) / NT);
   auto y_at = [&](int i) {
     return u < 0 ? row[i] : shr64((int64_t)((uint64_t)row[i] * (uint64_t)a.tnum), 16);
-  };
-  auto block_max = [&](int64_t v) {
-    for (int o = 16; o > 0; o >>= 1) { const int64_t w = __shfl_xor_sync(0xffffffffu, v, o); v = w > v ? w : v; }
-    __syncthreads();
-    if (lane == 0) red[warp] = (uint64_t)v;
-    __syncthreads();
-    for (int i = 0; i < TV_THREADS / 32; ++i) v = (int64_t)red[i] > v ? (int64_t)red[i] : v;
-    return v;
   };
   int64_t m = INT64_MIN;
   int first = INT32_MAX;
@@ -45,9 +41,12 @@ __global__ void __launch_bounds__(TV_THREADS) k_tree_sample(const VerArgs a) {
     const int64_t y = y_at(i);
     if (y > m || first == INT32_MAX) { m = y; first = i; }
   }
-  const int64_t M = block_max(m);
+  int64_t M = m;
+  for (int o = 16; o > 0; o >>= 1) { const int64_t w = __shfl_xor_sync(0xffffffffu, M, o); M = w > M ? w : M; }
+  if (lane == 0) red[warp] = (uint64_t)M;
   if (tid == 0) tok = a.V - 1;
   __syncthreads();
+  for (int i = 0; i < NT / 32; ++i) M = (int64_t)red[i] > M ? (int64_t)red[i] : M;
   if (u < 0) {
     if (m == M && first != INT32_MAX) atomicMin(&tok, first);
   } else {
@@ -58,20 +57,20 @@ __global__ void __launch_bounds__(TV_THREADS) k_tree_sample(const VerArgs a) {
     if (lane == 0) red[warp] = (uint64_t)s;
     __syncthreads();
     uint64_t S = 0;
-    for (int i = 0; i < TV_THREADS / 32; ++i) S += red[i];
+    for (int i = 0; i < NT / 32; ++i) S += red[i];
     auto p_at = [&](int i) { return ((uint64_t)tree_exp(a.exp_t, (uint64_t)M - (uint64_t)y_at(i)) << 20) / S; };
     int64_t ps = 0;
     for (int i = c0; i < c1; ++i) ps += (int64_t)p_at(i);
     scan[tid] = ps;
     __syncthreads();
-    for (int o = 1; o < TV_THREADS; o <<= 1) {
+    for (int o = 1; o < NT; o <<= 1) {
       const int64_t add = tid >= o ? scan[tid - o] : 0;
       __syncthreads();
       scan[tid] += add;
       __syncthreads();
     }
     const int64_t before = scan[tid] - ps;
-    const int64_t target = (int64_t)(((uint64_t)u * (uint64_t)scan[TV_THREADS - 1]) >> 20);
+    const int64_t target = (int64_t)(((uint64_t)u * (uint64_t)scan[NT - 1]) >> 20);
     if (before <= target && target < before + ps) {
       int64_t cum = before;
       for (int i = c0; i < c1; ++i) {
@@ -84,8 +83,190 @@ __global__ void __launch_bounds__(TV_THREADS) k_tree_sample(const VerArgs a) {
   if (tid == 0) a.sampled[r] = tok;
 }
 
+__global__ void __launch_bounds__(1024) k_tree_sample_long(const VerArgs a) { sample_row<1024>(a, blockIdx.x); }
+
+// A row by a cluster: CTA c holds a slice of up to 1024 IT logits in registers (two neighbouring ones a
+// thread and step), so the row is read once while the cluster agrees on its maximum and its sum.  What
+// stays is the scaled logit as 32 bits, then e, then p; the sum of all p is at most 2^20, so 32-bit sums
+// do from there.  A row with a scaled logit of 2^30 or more goes to sample_row instead.
+constexpr int TV_THREADS = 512;
+
+template <int IT>
+__global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(const VerArgs a, int slice) {
+  extern __shared__ __align__(128) unsigned char sm[];
+  int32_t* T = reinterpret_cast<int32_t*>(sm);
+  constexpr int NW = TV_THREADS / 32;
+  __shared__ int red[NW];
+  __shared__ uint64_t red64[NW];
+  __shared__ uint32_t seg[IT * NW];
+  __shared__ int lmax, lwide, lfirst;
+  __shared__ uint64_t lsum;
+  __shared__ uint32_t lps;
+  __shared__ uint64_t tbar;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), c = (int)cluster.block_rank();
+  const int r = (int)blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int i0 = c * slice, n = max(0, min(a.V - i0, slice));
+  const int64_t* row = a.logits + (int64_t)r * a.ld + i0;
+  const int u = a.u20[r];
+  if (tid == 0 && u >= 0) {
+    mbar_init(&tbar, 1);
+    mbar_fence_init();
+    mbar_expect_tx(&tbar, 40960);
+    bulk_g2s(T, a.exp_t, 40960, &tbar);
+  }
+  if (tid < EXP_LEN - 10240) T[10240 + tid] = a.exp_t[10240 + tid];
+  const bool pair = ((((uintptr_t)row) & 15) == 0);
+  int y[2 * IT];
+  int m = INT32_MIN;
+  bool big = false;
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int i = it * 2 * TV_THREADS + 2 * tid;
+    longlong2 v = make_longlong2(0, 0);
+    if (pair && i + 1 < n) v = __ldcs(reinterpret_cast<const longlong2*>(row + i));
+    else {
+      if (i < n) v.x = row[i];
+      if (i + 1 < n) v.y = row[i + 1];
+    }
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      const int64_t x = f ? v.y : v.x;
+      const int64_t s = u < 0 ? x : (int64_t)((uint64_t)x * (uint64_t)a.tnum + (1ull << 15)) >> 16;
+      big |= (uint64_t)(s + (1ll << 30)) >= (1ull << 31);
+      const int w = i + f < n ? (int)s : INT32_MIN;           // past the end: no term, never the maximum
+      y[2 * it + f] = w;
+      m = max(m, w);
+    }
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (lane == 0) red[warp] = m;
+  big = __syncthreads_or(big);
+  if (warp == 0) {
+    m = __reduce_max_sync(0xffffffffu, red[lane & (NW - 1)]);
+    if (lane == 0) { lmax = m; lwide = big; }
+  }
+  cluster.sync();
+  int M = INT32_MIN, wide = 0;
+  for (int cc = 0; cc < C; ++cc) {
+    M = max(M, *cluster.map_shared_rank(&lmax, cc));
+    wide |= *cluster.map_shared_rank(&lwide, cc);
+  }
+  if (wide) {
+    if (u >= 0 && !mbar_wait(&tbar, 0)) return;               // no copy is left in flight
+    if (c == 0) sample_row<TV_THREADS>(a, r);
+    cluster.sync();
+    return;
+  }
+  if (u < 0) {                                                // the lowest index of the maximum
+    int first = INT32_MAX;
+#pragma unroll
+    for (int k = 2 * IT - 1; k >= 0; --k)
+      if (y[k] == M) first = (k >> 1) * 2 * TV_THREADS + 2 * tid + (k & 1);
+    first = (int)__reduce_min_sync(0xffffffffu, (unsigned)first);
+    if (lane == 0) red[warp] = first;
+    __syncthreads();
+    if (warp == 0) {
+      first = (int)__reduce_min_sync(0xffffffffu, (unsigned)red[lane & (NW - 1)]);
+      if (lane == 0) lfirst = first == INT32_MAX ? first : first + i0;
+    }
+    cluster.sync();
+    if (c == 0 && tid == 0) {
+      int best = INT32_MAX;
+      for (int cc = 0; cc < C; ++cc) best = min(best, *cluster.map_shared_rank(&lfirst, cc));
+      a.sampled[r] = best;
+    }
+    cluster.sync();
+    return;
+  }
+  mbar_wait(&tbar, 0);
+  uint64_t s = 0;
+#pragma unroll
+  for (int k = 0; k < 2 * IT; ++k) {
+    const uint32_t e = y[k] == INT32_MIN ? 0u : exp_sm(T, (uint32_t)M - (uint32_t)y[k]);
+    y[k] = (int)e;
+    s += e;
+  }
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) red64[warp] = s;
+  __syncthreads();
+  if (tid == 0) {
+    s = 0;
+    for (int w = 0; w < NW; ++w) s += red64[w];
+    lsum = s;
+  }
+  cluster.sync();
+  uint64_t S = 0;
+  for (int cc = 0; cc < C; ++cc) S += *cluster.map_shared_rank(&lsum, cc);
+  const uint64_t inv = prob_inverse(S);
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    uint32_t p = 0;
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      const uint32_t e = (uint32_t)y[2 * it + f];
+      y[2 * it + f] = (int)(inv ? prob_of(e, inv) : prob_slow(e, S));
+      p += (uint32_t)y[2 * it + f];
+    }
+    p = __reduce_add_sync(0xffffffffu, p);                    // 64 neighbouring logits
+    if (lane == 0) seg[it * NW + warp] = p;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    uint32_t t = 0;
+    for (int k = lane; k < IT * NW; k += 32) t += seg[k];
+    t = __reduce_add_sync(0xffffffffu, t);
+    if (lane == 0) lps = t;
+  }
+  cluster.sync();
+  uint32_t total = 0, before = 0;
+  for (int cc = 0; cc < C; ++cc) {
+    const uint32_t t = *cluster.map_shared_rank(&lps, cc);
+    total += t;
+    before += cc < c ? t : 0;
+  }
+  const uint32_t target = (uint32_t)(((uint64_t)u * total) >> 20);
+  if (total == 0) {                                           // a row whose every p rounds to 0
+    if (c == 0 && tid == 0) a.sampled[r] = a.V - 1;
+  } else if (before <= target && target < before + lps) {     // one CTA: its segment, then its lane
+    // each warp scans the segments in order, 32 at a time; the segment's own warp goes on
+    int k = 0;
+    uint32_t at = before;
+    for (int k0 = 0; k0 < IT * NW; k0 += 32) {
+      const uint32_t x = k0 + lane < IT * NW ? seg[k0 + lane] : 0;
+      uint32_t inc = x;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const uint32_t w = __shfl_up_sync(0xffffffffu, inc, o); inc += lane >= o ? w : 0; }
+      const unsigned hit = __ballot_sync(0xffffffffu, at + inc > target);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        k = k0 + l;
+        at += __shfl_sync(0xffffffffu, inc - x, l);
+        break;
+      }
+      at += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (warp == k % NW) {
+      uint32_t pa = 0, pb = 0;
+#pragma unroll
+      for (int it = 0; it < IT; ++it)
+        if (it == k / NW) { pa = (uint32_t)y[2 * it]; pb = (uint32_t)y[2 * it + 1]; }
+      uint32_t inc = pa + pb;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const uint32_t w = __shfl_up_sync(0xffffffffu, inc, o); inc += lane >= o ? w : 0; }
+      const unsigned hit = __ballot_sync(0xffffffffu, at + inc > target);
+      if (lane == __ffs(hit) - 1) {
+        const bool first = at + inc - pb > target;
+        a.sampled[r] = i0 + (k / NW) * 2 * TV_THREADS + 2 * tid + (first ? 0 : 1);
+      }
+    }
+  }
+  cluster.sync();                                             // the peers' words stay until they are read
+}
+
 // One warp per sequence walks from node 0: 32 candidates at a time, the lowest one that fits.
 __global__ void __launch_bounds__(32) k_tree_walk(const VerArgs a) {
+  pdl_wait();
   const int b = blockIdx.x, lane = threadIdx.x;
   int r0 = a.row_start[b], r1 = a.row_start[b + 1];
   if (r0 < 0 || r1 > a.R || r1 < r0) r1 = r0 = 0;
@@ -112,10 +293,57 @@ __global__ void __launch_bounds__(32) k_tree_walk(const VerArgs a) {
   if (lane == 0) a.n[b] = len;
 }
 
+template <int IT>
+static cudaError_t launch_sample_rows(const VerArgs& a, int C, cudaStream_t st) {
+  static DevOnce attr_set;
+  if (!attr_set.done()) {
+    cudaError_t e = cudaFuncSetAttribute(k_tree_sample<IT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 41024);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_tree_sample<IT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    attr_set.set();
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)C * (unsigned)a.R);
+  cfg.blockDim = dim3(TV_THREADS);
+  cfg.dynamicSmemBytes = 41024;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)C;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_tree_sample<IT>, a, (a.V + 2 * C - 1) / (2 * C) * 2);
+}
+
 static cudaError_t launch_tree_verify(const VerArgs& a, cudaStream_t st) {
-  if (a.R) k_tree_sample<<<a.R, TV_THREADS, 0, st>>>(a);
-  if (a.B) k_tree_walk<<<a.B, 32, 0, st>>>(a);
-  return cudaGetLastError();
+  if (a.R) {
+    cudaError_t e;
+    // slices of a row over 8 CTAs, as few steps of 1024 logits as hold them
+    const int per = (a.V + 8191) / 8192;
+    if (per <= 2) e = launch_sample_rows<2>(a, 8, st);
+    else if (per <= 8) e = launch_sample_rows<8>(a, 8, st);
+    else if (per <= 20) e = launch_sample_rows<20>(a, 8, st);
+    else if (per <= 40) e = launch_sample_rows<20>(a, 16, st);
+    else {
+      k_tree_sample_long<<<a.R, 1024, 0, st>>>(a);
+      e = cudaGetLastError();
+    }
+    if (e != cudaSuccess) return e;
+  }
+  if (a.B) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.B);
+    cfg.blockDim = dim3(32);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_tree_walk, a);
+  }
+  return cudaSuccess;
 }
 
 }  // namespace exb
@@ -130,6 +358,7 @@ extern "C" int exb_tree_verify(const int64_t* logits, int64_t ld, int R, int V, 
   if (R < 0 || B < 0 || V < 1 || max_len < 1) return fail("R, B >= 0 and V, max_len >= 1");
   if (ld < V) return fail("row stride below V");
   if (tnum < 1 || tnum > (1ll << 32)) return fail("temperature multiplier in [1, 2^32]");
+  if ((uintptr_t)exp_t & 15) return fail("exp_t must be 16-byte aligned");
   if (!exp_t || (R && (!logits || !u20 || !tokens || !parent || !sampled)) ||
       (B && (!row_start || !n || !path || !out_tokens)))
     return fail("null argument");

@@ -5,6 +5,20 @@
 
 namespace exb {
 
+// n / d for 0 <= n < 2^30 by one multiplication: m = floor(2^(32+s) / d) + 1 with s = floor(log2 d), so
+// n * (m d - 2^(32+s)) < 2^30 * 2^(s+1) stays below 2^(32+s) and the quotient is exact; m = 0: a power of two
+struct FastDiv {
+  uint32_t m = 0;
+  int s = 0;
+};
+inline FastDiv fast_div(int d) {
+  FastDiv f;
+  while ((d >> f.s) > 1) ++f.s;
+  f.m = (d & (d - 1)) ? (uint32_t)((1ull << (32 + f.s)) / (uint32_t)d) + 1 : 0;
+  return f;
+}
+EXB_DEV int div_by(int n, FastDiv f) { return (int)((f.m ? __umulhi((uint32_t)n, f.m) : (uint32_t)n) >> f.s); }
+
 // Arguments of the tree attention kernels (see exb_tree_attention).
 struct TreeArgs {
   exb_kv_view kv;
@@ -20,6 +34,7 @@ struct TreeArgs {
   int R = 0, H = 0, rep = 0, B = 0, MP = 0, W = 0;
   int64_t cap = 0;                       // positions a table row can name: MP * page
   int64_t inv = 0;                       // round(2^16 / sqrt(hd))
+  FastDiv page_div;
 };
 
 // One sequence's rows and positions, cut to what the arguments can hold.
@@ -45,13 +60,89 @@ EXB_DEV TreeSeq tree_seq(const TreeArgs& a, int b, bool report) {
 }
 
 // page of position pos, or -1 (reported) where the table names none
-EXB_DEV int page_of(const exb_kv_view& kv, const int32_t* __restrict__ row, int pos, int& off, int32_t* status) {
-  const int i = pos / kv.page;
-  off = pos - i * kv.page;
-  const int pg = row[i];
-  if ((unsigned)pg < (unsigned)kv.pages) return pg;
-  set_err(status, ERR_BOUNDS);
+EXB_DEV int page_of(const TreeArgs& a, const int32_t* __restrict__ row, int pos, int& off) {
+  const int i = div_by(pos, a.page_div);
+  off = pos - i * a.kv.page;
+  const int pg = __ldg(row + i);
+  if ((unsigned)pg < (unsigned)a.kv.pages) return pg;
+  set_err(a.status, ERR_BOUNDS);
   return -1;
+}
+EXB_DEV const int16_t* k_row(const exb_kv_view& kv, int head, int pg, int off) {
+  return kv.k + (int64_t)pg * kv.k_page + (int64_t)head * kv.k_head + (int64_t)off * kv.k_pos;
+}
+EXB_DEV const int32_t* v_row(const exb_kv_view& kv, int head, int pg, int off) {
+  return kv.v + (int64_t)pg * kv.v_page + (int64_t)head * kv.v_head + (int64_t)off * kv.v_pos;
+}
+EXB_DEV int k_shift(const exb_kv_view& kv, int head, int pg, int off) {
+  return kv.ks[(int64_t)pg * kv.s_page + (int64_t)head * kv.s_head + (int64_t)off * kv.s_pos];
+}
+
+// p = (e << 20) // sum for 0 <= e <= 2^24 by two multiplications: inv = ceil(2^86 / sum), and
+// e * (inv * sum - 2^86) < 2^24 * 2^42 = 2^66, so (e * inv) >> 66 is the exact quotient for
+// 2^24 <= sum < 2^42 (the row's largest term alone is 2^24; 2^18 positions).  Other sums: inv = 0, and
+// the division itself.
+EXB_DEV uint64_t prob_inverse(uint64_t sum) {
+  if (sum < (1ull << 24) || sum >= (1ull << 42)) return 0;
+  const uint64_t a = 1ull << 62;
+  const uint64_t q0 = a / sum, r0 = a - q0 * sum;
+  const uint64_t q1 = (r0 << 12) / sum, r1 = (r0 << 12) - q1 * sum;
+  const uint64_t q2 = (r1 << 12) / sum, r2 = (r1 << 12) - q2 * sum;
+  return (q0 << 24) + (q1 << 12) + q2 + (r2 ? 1 : 0);
+}
+EXB_DEV uint32_t prob_of(uint32_t e, uint64_t inv) {
+  const uint64_t t = (uint64_t)e * (uint32_t)inv;
+  const uint64_t h = (uint64_t)e * (uint32_t)(inv >> 32) + (t >> 32);
+  return (uint32_t)(h >> 34);
+}
+EXB_DEV uint32_t prob_slow(uint32_t e, uint64_t sum) { return sum ? (uint32_t)(((uint64_t)e << 20) / sum) : 0u; }
+
+// the table value at distance d, from a copy of the table in shared memory
+EXB_DEV uint32_t exp_sm(const int32_t* T, uint32_t d) {
+  if (d >= (40u << 16)) return 0;
+  const int a = T[d >> 8], b = T[(d >> 8) + 1];
+  return (uint32_t)(a - (((a - b) * (int)(d & 255) + 128) >> 8));
+}
+
+// 8 int16 -> their low bytes (unsigned digits) and high bytes (signed digits), in order
+EXB_DEV void int16_digits(const int4 v, uint2& lo, uint2& hi) {
+  lo = make_uint2(__byte_perm((uint32_t)v.x, (uint32_t)v.y, 0x6420), __byte_perm((uint32_t)v.z, (uint32_t)v.w, 0x6420));
+  hi = make_uint2(__byte_perm((uint32_t)v.x, (uint32_t)v.y, 0x7531), __byte_perm((uint32_t)v.z, (uint32_t)v.w, 0x7531));
+}
+// byte planes of four words: o[i] = byte i of a, b, c, d in order
+EXB_DEV void byte_planes(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t* o) {
+  const uint32_t l0 = __byte_perm(a, b, 0x5140), l1 = __byte_perm(c, d, 0x5140);
+  const uint32_t h0 = __byte_perm(a, b, 0x7362), h1 = __byte_perm(c, d, 0x7362);
+  o[0] = __byte_perm(l0, l1, 0x5410);
+  o[1] = __byte_perm(l0, l1, 0x7632);
+  o[2] = __byte_perm(h0, h1, 0x5410);
+  o[3] = __byte_perm(h0, h1, 0x7632);
+}
+
+// D += A (16 x 32) . B (32 x 8) in int8 digits, signed or not by operand, int32 sums
+template <bool AS, bool BS>
+EXB_DEV void mma_digits(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (!AS && !BS)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else if constexpr (!AS && BS)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else if constexpr (AS && !BS)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+EXB_DEV int64_t mad_wide_s32(int a, int b, int64_t t) {
+  int64_t d;
+  asm("mad.wide.s32 %0, %1, %2, %3;" : "=l"(d) : "r"(a), "r"(b), "l"(t));
+  return d;
+}
+// low word of a 64-bit arithmetic shift right by n in [0, 32]
+EXB_DEV int shift_low(int64_t x, int n) {
+  return (int)__funnelshift_rc((uint32_t)x, (uint32_t)((uint64_t)x >> 32), n);
 }
 
 // exp table at d = max - score (exact_llm.py:109-115).  d is not negative unless the difference left
