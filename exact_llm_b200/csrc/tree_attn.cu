@@ -37,7 +37,8 @@ struct TreeGeo {
   static constexpr int KP = 8 / DG;                          // warps that share a dim group: key parts
   static constexpr int KS = HD < 32 ? 1 : HD / 32;           // 32-dim steps of a score
   static constexpr int OUT = KP * NR * HD;                   // partial outputs (int64)
-  static size_t smem(int ldk) { return 41024 + (size_t)OUT * 8 + (size_t)NR * ldk * 4; }
+  // exp table, partial outputs, score rows, the V rows' places
+  static size_t smem(int ldk) { return 41024 + (size_t)OUT * 8 + (size_t)(NR + 1) * ldk * 4; }
 };
 // score row pitch for n positions: 4 mod 16 words, so a warp's stores and loads hit 32 banks
 inline int tree_pitch(int64_t n) { return (int)((n + 15) / 16 * 16 + 4); }
@@ -50,9 +51,10 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
   int32_t* T = reinterpret_cast<int32_t*>(sm);                               // exp table
   int64_t* pout = reinterpret_cast<int64_t*>(sm + 41024);                    // KP x NR x HD
   int32_t* sc = reinterpret_cast<int32_t*>(sm + 41024 + (size_t)G::OUT * 8); // NR x ldk
+  uint32_t* vat = reinterpret_cast<uint32_t*>(sc + (size_t)NR * ldk);        // V row of every position, in 16 bytes
   __shared__ int64_t lmax[NR], lsum[NR];
   __shared__ int64_t wmax[8][NR];
-  __shared__ uint64_t pinv[NR], psum[NR];
+  __shared__ uint64_t pinv[NR];
   __shared__ int32_t base[NR];
   __shared__ int qsh[NR];
   __shared__ const uint64_t* rmask[NR];
@@ -115,7 +117,7 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
     mbar_expect_tx(&tbar, EXP_BULK);
     bulk_g2s(T, a.exp_t, EXP_BULK, &tbar);
   }
-  if (tid < EXP_LEN - EXP_BULK / 4) T[EXP_BULK / 4 + tid] = a.exp_t[EXP_BULK / 4 + tid];
+  if (tid < EXP_LEN - EXP_BULK / 4) T[EXP_BULK / 4 + tid] = 0;       // from 40.0 on (exp_sm_flat)
   const int32_t* trow = a.table + (size_t)b * a.MP;
   const int g0 = find[1] * NR, ng = min(NR, sq.T * a.rep - g0);
   // row i of the tile: node (g0 + i) / rep, head (g0 + i) % rep of the group
@@ -166,33 +168,49 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
   // Where some shift is outside, the CTA goes over its keys twice: maxima, then clamped distances.
   const int c2 = (int)(a.inv << 16), c1 = (int)(a.inv << 8), c0 = (int)a.inv;
   int64_t mx[NT][2];
+  int mx32[NT][2];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = INT64_MIN;
+  for (int nt = 0; nt < NT; ++nt) mx32[nt][0] = mx32[nt][1] = INT32_MIN;
+  // one step's keys, fetched a step ahead
+  struct Keys {
+    int4 k[2][G::KS];
+    int sh[2];                                               // -1: no such key
+  };
+  auto fetch = [&](int u, Keys& x, bool store) {
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      const int t = u + g + 8 * f;
+      int off = 0;
+      const int pg = t < n ? page_of(a, trow, t0 + t, off) : -1;
+      x.sh[f] = -1;
+#pragma unroll
+      for (int ks = 0; ks < G::KS; ++ks) x.k[f][ks] = make_int4(0, 0, 0, 0);
+      if (pg >= 0) {
+        const int16_t* kr = k_row(kv, j, pg, off);
+#pragma unroll
+        for (int ks = 0; ks < G::KS; ++ks)
+          if (ks * 32 + 8 * tq < HD) x.k[f][ks] = *reinterpret_cast<const int4*>(kr + ks * 32 + 8 * tq);
+        x.sh[f] = (uint8_t)k_shift(kv, j, pg, off);
+      }
+      if (store && tq == 0) {                                // V is needed after the exchanges: into L2 now
+        const int32_t* vr = v_row(kv, j, max(pg, 0), off);
+        if (pg >= 0) prefetch_l2_bulk(vr, HD * 4);
+        vat[t] = pg >= 0 ? (uint32_t)((vr - kv.v) >> 2) : 0u;        // a key that is not there has p = 0
+      }
+    }
+  };
   // one sweep over the keys: `wide` scores in 64 bits, `store` into sc
   auto sweep = [&](auto wide_t, bool store, bool track) {
     constexpr bool wide = decltype(wide_t)::value;
     bool fits = true;
+    Keys next;
+    if (warp * 16 < n) fetch(warp * 16, next, store);
+#pragma unroll 1
     for (int u = warp * 16; u < n; u += 128) {
-      int sh[2], pgs[2];
-      const int16_t* kr[2];
-#pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const int t = u + g + 8 * f;
-        int off = 0;
-        pgs[f] = t < n ? page_of(a, trow, t0 + t, off) : -1;
-        kr[f] = k_row(kv, j, max(pgs[f], 0), off);
-        sh[f] = pgs[f] >= 0 ? k_shift(kv, j, pgs[f], off) : 0;
-        if (store && pgs[f] >= 0 && tq == 0)                 // V is needed after the exchanges: into L2 now
-          prefetch_l2_bulk(v_row(kv, j, pgs[f], off), HD * 4);
-      }
-      if (!wide) fits &= sh[0] + qmax <= 13 && sh[1] + qmax <= 13 && sh[0] >= 0 && sh[1] >= 0;
-      int4 kk[2][G::KS];
-#pragma unroll
-      for (int f = 0; f < 2; ++f)
-#pragma unroll
-        for (int ks = 0; ks < G::KS; ++ks)
-          kk[f][ks] = pgs[f] >= 0 && ks * 32 + 8 * tq < HD ? *reinterpret_cast<const int4*>(kr[f] + ks * 32 + 8 * tq)
-                                                            : make_int4(0, 0, 0, 0);
+      const Keys x = next;
+      if (u + 128 < n) fetch(u + 128, next, store);
+      const int sh[2] = {max(x.sh[0], 0), max(x.sh[1], 0)};
+      if (!wide) fits &= sh[0] + qmax <= 13 && sh[1] + qmax <= 13;
       int ll[NT][4], md[NT][4], hh[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -201,8 +219,8 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
 #pragma unroll
       for (int ks = 0; ks < G::KS; ++ks) {
         uint2 l0, h0, l1, h1;
-        int16_digits(kk[0][ks], l0, h0);
-        int16_digits(kk[1][ks], l1, h1);
+        int16_digits(x.k[0][ks], l0, h0);
+        int16_digits(x.k[1][ks], l1, h1);
         const uint32_t al[4] = {l0.x, l1.x, l0.y, l1.y}, ah[4] = {h0.x, h1.x, h0.y, h1.y};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -212,24 +230,27 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
           mma_digits<true, true>(hh[nt], ah, qh[nt][ks][0], qh[nt][ks][1]);
         }
       }
-      const bool tree = t0 + u + 15 >= sq.ctx;
+      const bool all = __all_sync(0xffffffffu, x.sh[0] >= 0 && x.sh[1] >= 0) && t0 + u + 15 < sq.ctx;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
           const int kf = f >> 1, i = nt * 8 + 2 * tq + (f & 1), t = u + g + 8 * kf;
-          bool see = pgs[kf] >= 0;
-          if (tree && see && t0 + t >= sq.ctx) {
-            const int node = t0 + t - sq.ctx;
-            see = (rmask[i][node >> 6] >> (node & 63)) & 1;
+          bool see = true;
+          if (!all) {
+            see = x.sh[kf] >= 0;
+            if (see && t0 + t >= sq.ctx) {
+              const int node = t0 + t - sq.ctx;
+              see = (rmask[i][node >> 6] >> (node & 63)) & 1;
+            }
           }
           const int sft = 32 - qs_r[nt][f & 1] - sh[kf];
           if (!wide) {
-            const int64_t x = mad_wide_s32(hh[nt][f], c2, mad_wide_s32(md[nt][f], c1, mad_wide_s32(ll[nt][f], c0,
-                                                                        (int64_t)(1ull << ((sft - 1) & 63)))));
-            const int s = shift_low(x, sft);
-            if (see && s > mx[nt][f & 1]) mx[nt][f & 1] = s;
-            sc[i * ldk + t] = see ? s : INT32_MIN;
+            const int64_t w = mad_wide_s32(hh[nt][f], c2, mad_wide_s32(md[nt][f], c1, mad_wide_s32(ll[nt][f], c0,
+                                                                        (int64_t)(1u << ((sft - 1) & 31)))));
+            const int s = see ? shift_low(w, sft) : INT32_MIN;
+            mx32[nt][f & 1] = max(mx32[nt][f & 1], s);
+            sc[i * ldk + t] = s;
           } else {
             const int64_t acc = mad_wide_s32(hh[nt][f], 65536, mad_wide_s32(md[nt][f], 256, (int64_t)ll[nt][f]));
             const int64_t s = shr64((int64_t)((uint64_t)acc * (uint64_t)a.inv), sft);
@@ -263,6 +284,7 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
     }
     __syncthreads();
   };
+  const unsigned live = NR * C - (tid & ~31) >= 32 ? 0xffffffffu : (1u << max(NR * C - (tid & ~31), 0)) - 1u;   // lanes below NR C
   const bool fits = sweep(std::false_type{}, true, true);
   const bool wide = __syncthreads_or(!fits || qneg);
   if (wide) {
@@ -272,23 +294,32 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
     cta_max();
     sweep(std::true_type{}, true, false);
   } else {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int f = 0; f < 2; ++f) mx[nt][f] = mx32[nt][f] == INT32_MIN ? INT64_MIN : mx32[nt][f];
     cta_max();
   }
   // hidden rows of the tail, so that the loops below take whole steps of 32
-  for (int e = tid; e < NR * (n32 - n); e += TC_THREADS_T) {
-    const int i = e / (n32 - n);
-    sc[i * ldk + n + e - i * (n32 - n)] = INT32_MIN;
+  for (int e = tid; e < (NR + 1) * (n32 - n); e += TC_THREADS_T) {
+    const int i = e / (n32 - n), t = n + e - i * (n32 - n);
+    if (i < NR) sc[i * ldk + t] = INT32_MIN;
+    else vat[t] = 0;
   }
   cluster.sync();
-  if (tid < NR) {
-    int64_t m = INT64_MIN;
-    for (int cc = 0; cc < C; ++cc) { const int64_t w = cluster.map_shared_rank(lmax, cc)[tid]; m = w > m ? w : m; }
+  // thread (row, peer): every peer's word at once, then over the C lanes of the row (C a power of two)
+  if (tid < NR * C) {
+    const int i = tid / C;
+    int64_t m = cluster.map_shared_rank(lmax, tid & (C - 1))[i];
+    for (int o = 1; o < C; o <<= 1) { const int64_t w = __shfl_xor_sync(live, m, o); m = w > m ? w : m; }
     // distance of a stored score: base - sc as 32 bits without a sign
-    if (wide) {
-      const uint64_t d = (uint64_t)m - (uint64_t)lmax[tid];
-      base[tid] = d < (1ull << 30) ? (int)d : (1 << 30);
-    } else {
-      base[tid] = m > INT32_MAX ? INT32_MAX : (int)m;        // another CTA's row may be far above
+    if ((tid & (C - 1)) == 0) {
+      if (wide) {
+        const uint64_t d = (uint64_t)m - (uint64_t)lmax[i];
+        base[i] = d < (1ull << 30) ? (int)d : (1 << 30);
+      } else {
+        base[i] = m > INT32_MAX ? INT32_MAX : (int)m;        // another CTA's row may be far above
+      }
     }
   }
   if (!mbar_wait(&tbar, 0)) set_err(a.status, ERR_WAIT_TIMEOUT);             // the table
@@ -299,8 +330,8 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
     int64_t s = 0;
     const int bs = base[i];
     for (int t = lane; t < n32; t += 32) {
-      const int v = sc[i * ldk + t];
-      const uint32_t e = v == INT32_MIN ? 0u : exp_sm(T, (uint32_t)bs - (uint32_t)v);
+      // a hidden position (INT32_MIN) is at 2^29 or more from any base: e = 0
+      const uint32_t e = exp_sm_flat(T, (uint32_t)bs - (uint32_t)sc[i * ldk + t]);
       sc[i * ldk + t] = (int)e;
       s += e;
     }
@@ -309,11 +340,10 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
     if (lane == 0) lsum[i] = s;
   }
   cluster.sync();
-  if (tid < NR) {
-    uint64_t s = 0;
-    for (int cc = 0; cc < C; ++cc) s += (uint64_t)cluster.map_shared_rank(lsum, cc)[tid];
-    psum[tid] = s;
-    pinv[tid] = prob_inverse(s);
+  if (tid < NR * C) {
+    uint64_t s = (uint64_t)cluster.map_shared_rank(lsum, tid & (C - 1))[tid / C];
+    for (int o = 1; o < C; o <<= 1) s += __shfl_xor_sync(live, s, o);
+    if ((tid & (C - 1)) == 0) pinv[tid / C] = prob_inverse(s);       // 0 for a row that sees nothing: p = 0
   }
   __syncthreads();
   // ---- phase 3: out += p . v.  Warp: 32 dims (its group) x every KP-th step of 32 positions.  Operand
@@ -331,17 +361,14 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
         for (int w = 0; w < 6; ++w)
 #pragma unroll
           for (int f = 0; f < 4; ++f) acc[nt][mt][w][f] = 0;
-    uint64_t inv[NT], sum[NT];
+    uint64_t inv[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) { inv[nt] = pinv[nt * 8 + g]; sum[nt] = psum[nt * 8 + g]; }
+    for (int nt = 0; nt < NT; ++nt) inv[nt] = pinv[nt * 8 + g];
+    const int4* vbase = reinterpret_cast<const int4*>(kv.v) + (dlive ? dg * 8 + g : 0);
     auto load_v = [&](int u, int4* v) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int t = u + tq + 4 * i;
-        int off = 0;
-        const int pg = t < n ? page_of(a, trow, t0 + t, off) : -1;
-        v[i] = pg >= 0 && dlive ? __ldg(reinterpret_cast<const int4*>(v_row(kv, j, pg, off) + dg * 32 + 4 * g))
-                                : make_int4(0, 0, 0, 0);
+        v[i] = __ldg(vbase + vat[u + tq + 4 * i]);           // past the CTA's keys p is 0
       }
     };
     int4 v[8];
@@ -370,7 +397,7 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint32_t e = (uint32_t)sc[(nt * 8 + g) * ldk + u + tq + 16 * h + 4 * i];
-            p[i] = inv[nt] ? prob_of(e, inv[nt]) : prob_slow(e, sum[nt]);
+            p[i] = prob_of(e, inv[nt]);
           }
           byte_planes(p[0], p[1], p[2], p[3], pb[h]);
         }
@@ -412,7 +439,13 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
   const int tot = ng * HD, per = (tot + C - 1) / C;
   for (int e = c * per + tid; e < min(tot, (c + 1) * per); e += TC_THREADS_T) {
     int64_t s = 0;
-    for (int cc = 0; cc < C; ++cc) s += cluster.map_shared_rank(pout, cc)[e];
+    for (int c0 = 0; c0 < C; c0 += 8) {
+      int64_t w[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = c0 + k < C ? cluster.map_shared_rank(pout, c0 + k)[e] : 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += w[k];
+    }
     const int i = e / HD;
     a.out[q_index(i) * HD + (e - i * HD)] = shr64(s, 20);
   }
@@ -533,6 +566,11 @@ static cudaError_t launch_cluster_hd(const TreeArgs& a, int C, int ldk, cudaStre
   }
 }
 
+// elements from the first V row of a layer to behind its last
+static int64_t v_extent(const exb_kv_view& kv) {
+  return (kv.pages - 1) * std::abs(kv.v_page) + (kv.KV - 1) * std::abs(kv.v_head) + (kv.page - 1) * std::abs(kv.v_pos) + kv.hd;
+}
+
 static cudaError_t launch_tree_attention(const TreeArgs& a, cudaStream_t st) {
   // rows per tile: 16 where the trees have that many in a group
   const int NT = (int64_t)a.R * a.rep > 8ll * a.B ? 2 : 1, NR = 8 * NT;
@@ -540,14 +578,14 @@ static cudaError_t launch_tree_attention(const TreeArgs& a, cudaStream_t st) {
   // or a long score array), each with 64 positions at least; more where the scores need the room
   const int64_t clusters = std::max<int64_t>(a.B, ((int64_t)a.R * a.rep + NR - 1) / NR) * a.kv.KV;
   auto pitch = [&](int c) { return tree_pitch(((a.cap + c - 1) / c + 31) / 16 * 16); };
-  auto smem_of = [&](int c) { return 41024 + (size_t)2048 * NR + (size_t)NR * pitch(c) * 4; };
+  auto smem_of = [&](int c) { return 41024 + (size_t)2048 * NR + (size_t)(NR + 1) * pitch(c) * 4; };
   int C = 1;
   while (C < 16 && (smem_of(C) > (size_t)TREE_SMEM_MAX ||
                     ((int64_t)C * 64 < a.cap && clusters * 2 * C <= (NT == 2 || smem_of(2 * C) > 110 * 1024 ? 148 : 296))))
     C *= 2;
   const size_t smem = smem_of(C);
   const int ldk = pitch(C);
-  if (smem <= (size_t)TREE_SMEM_MAX)
+  if (smem <= (size_t)TREE_SMEM_MAX && v_extent(a.kv) < (1ll << 34))       // V places: 32 bits of 16 bytes
     return NT == 2 ? launch_cluster_hd<2>(a, C, ldk, st) : launch_cluster_hd<1>(a, C, ldk, st);
   k_tree_simple<<<dim3(a.R, a.H), TS_THREADS, 0, st>>>(a);
   return cudaGetLastError();

@@ -24,7 +24,7 @@ struct VerArgs {
 // A row by one CTA of NT threads that reads it again for every step: any length, any values.
 // Thread t owns the t-th of NT contiguous slices of the row.
 template <int NT>
-EXB_DEV void sample_row(const VerArgs& a, int r) {
+__device__ __noinline__ void sample_row(const VerArgs& a, int r) {
   __shared__ uint64_t red[NT / 32];
   __shared__ int64_t scan[NT];
   __shared__ int tok;
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(con
   __shared__ uint64_t red64[NW];
   __shared__ uint32_t seg[IT * NW];
   __shared__ int lmax, lwide, lfirst;
-  __shared__ uint64_t lsum;
+  __shared__ uint64_t lsum, linv;
   __shared__ uint32_t lps;
   __shared__ uint64_t tbar;
   cg::cluster_group cluster = cg::this_cluster();
@@ -115,43 +115,58 @@ __global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(con
     mbar_expect_tx(&tbar, 40960);
     bulk_g2s(T, a.exp_t, 40960, &tbar);
   }
-  if (tid < EXP_LEN - 10240) T[10240 + tid] = a.exp_t[10240 + tid];
+  if (tid < EXP_LEN - 10240) T[10240 + tid] = 0;              // from 40.0 on (exp_sm_flat)
   const bool pair = ((((uintptr_t)row) & 15) == 0);
+  // a logit of 32 bits times tnum < 2^31, scaled; `big` gathers what leaves the range (|y| < 2^30)
+  const int tn = u < 0 ? 1 << 16 : (int)a.tnum;
   int y[2 * IT];
   int m = INT32_MIN;
-  bool big = false;
+  uint32_t big = 0;
+  auto scaled = [&](long long x) {
+    const int lo = (int)x, hi = (int)(x >> 32);
+    const int64_t w = mad_wide_s32(lo, tn, 1 << 15);
+    const int wh = (int)(w >> 32);
+    big |= (uint32_t)(hi ^ (lo >> 31)) | ((uint32_t)(wh + (1 << 14)) >> 15);
+    return (int)__funnelshift_r((uint32_t)w, (uint32_t)wh, 16);
+  };
+  constexpr int NB = IT < 4 ? IT : 4;                         // loads in flight a thread
 #pragma unroll
-  for (int it = 0; it < IT; ++it) {
-    const int i = it * 2 * TV_THREADS + 2 * tid;
-    longlong2 v = make_longlong2(0, 0);
-    if (pair && i + 1 < n) v = __ldcs(reinterpret_cast<const longlong2*>(row + i));
-    else {
-      if (i < n) v.x = row[i];
-      if (i + 1 < n) v.y = row[i + 1];
+  for (int it0 = 0; it0 < IT; it0 += NB) {
+    longlong2 v[NB];
+    const bool full = (it0 + NB) * 2 * TV_THREADS <= n;
+    const int64_t* at = row + it0 * 2 * TV_THREADS + 2 * tid;
+    if (full && pair) {
+#pragma unroll
+      for (int k = 0; k < NB; ++k) v[k] = __ldcs(reinterpret_cast<const longlong2*>(at + k * 2 * TV_THREADS));
+    } else {
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        const int i = (it0 + k) * 2 * TV_THREADS + 2 * tid;
+        v[k].x = i < n ? row[i] : 0;
+        v[k].y = i + 1 < n ? row[i + 1] : 0;
+      }
     }
 #pragma unroll
-    for (int f = 0; f < 2; ++f) {
-      const int64_t x = f ? v.y : v.x;
-      const int64_t s = u < 0 ? x : (int64_t)((uint64_t)x * (uint64_t)a.tnum + (1ull << 15)) >> 16;
-      big |= (uint64_t)(s + (1ll << 30)) >= (1ull << 31);
-      const int w = i + f < n ? (int)s : INT32_MIN;           // past the end: no term, never the maximum
-      y[2 * it + f] = w;
-      m = max(m, w);
+    for (int k = 0; k < NB; ++k) {
+      const int i = (it0 + k) * 2 * TV_THREADS + 2 * tid;
+      const int y0 = scaled(v[k].x), y1 = scaled(v[k].y);     // past the end: no term, never the maximum
+      y[2 * (it0 + k)] = full || i < n ? y0 : INT32_MIN;
+      y[2 * (it0 + k) + 1] = full || i + 1 < n ? y1 : INT32_MIN;
+      m = max(m, max(y[2 * (it0 + k)], y[2 * (it0 + k) + 1]));
     }
   }
   m = __reduce_max_sync(0xffffffffu, m);
   if (lane == 0) red[warp] = m;
-  big = __syncthreads_or(big);
+  const int any_big = __syncthreads_or(big != 0);
   if (warp == 0) {
     m = __reduce_max_sync(0xffffffffu, red[lane & (NW - 1)]);
-    if (lane == 0) { lmax = m; lwide = big; }
+    if (lane == 0) { lmax = m; lwide = any_big; }
   }
   cluster.sync();
-  int M = INT32_MIN, wide = 0;
-  for (int cc = 0; cc < C; ++cc) {
-    M = max(M, *cluster.map_shared_rank(&lmax, cc));
-    wide |= *cluster.map_shared_rank(&lwide, cc);
-  }
+  // every warp reads all peers' words at once, one a lane
+  const int peer = lane & (C - 1);
+  const int M = __reduce_max_sync(0xffffffffu, *cluster.map_shared_rank(&lmax, peer));
+  const bool wide = __any_sync(0xffffffffu, *cluster.map_shared_rank(&lwide, peer));
   if (wide) {
     if (u >= 0 && !mbar_wait(&tbar, 0)) return;               // no copy is left in flight
     if (c == 0) sample_row<TV_THREADS>(a, r);
@@ -171,41 +186,50 @@ __global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(con
       if (lane == 0) lfirst = first == INT32_MAX ? first : first + i0;
     }
     cluster.sync();
-    if (c == 0 && tid == 0) {
-      int best = INT32_MAX;
-      for (int cc = 0; cc < C; ++cc) best = min(best, *cluster.map_shared_rank(&lfirst, cc));
-      a.sampled[r] = best;
+    if (c == 0 && warp == 0) {
+      const int best = __reduce_min_sync(0xffffffffu, *cluster.map_shared_rank(&lfirst, peer));
+      if (lane == 0) a.sampled[r] = best;
     }
     cluster.sync();
     return;
   }
   mbar_wait(&tbar, 0);
-  uint64_t s = 0;
+  uint32_t es = 0;                                            // at most 2^24 each, 40 a thread
 #pragma unroll
   for (int k = 0; k < 2 * IT; ++k) {
-    const uint32_t e = y[k] == INT32_MIN ? 0u : exp_sm(T, (uint32_t)M - (uint32_t)y[k]);
+    const uint32_t e = exp_sm_flat(T, (uint32_t)M - (uint32_t)y[k]);
     y[k] = (int)e;
-    s += e;
+    es += e;
   }
+  uint64_t s = es;
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane == 0) red64[warp] = s;
   __syncthreads();
-  if (tid == 0) {
-    s = 0;
-    for (int w = 0; w < NW; ++w) s += red64[w];
-    lsum = s;
+  if (warp == 0) {
+    s = lane < NW ? red64[lane] : 0;
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) lsum = s;
   }
   cluster.sync();
-  uint64_t S = 0;
-  for (int cc = 0; cc < C; ++cc) S += *cluster.map_shared_rank(&lsum, cc);
-  const uint64_t inv = prob_inverse(S);
+  if (warp == 0) {                                            // the reciprocal once, not by every thread
+    uint64_t S = lane < C ? *cluster.map_shared_rank(&lsum, lane) : 0;
+    for (int o = 16; o > 0; o >>= 1) S += __shfl_xor_sync(0xffffffffu, S, o);
+    if (lane == 0) linv = prob_inverse(S);
+  }
+  __syncthreads();
+  const uint64_t inv = linv;
+  if (!inv) {                                                 // a sum past the reciprocal's range
+    if (c == 0) sample_row<TV_THREADS>(a, r);
+    cluster.sync();
+    return;
+  }
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
     uint32_t p = 0;
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
       const uint32_t e = (uint32_t)y[2 * it + f];
-      y[2 * it + f] = (int)(inv ? prob_of(e, inv) : prob_slow(e, S));
+      y[2 * it + f] = (int)prob_of(e, inv);
       p += (uint32_t)y[2 * it + f];
     }
     p = __reduce_add_sync(0xffffffffu, p);                    // 64 neighbouring logits
@@ -219,12 +243,9 @@ __global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(con
     if (lane == 0) lps = t;
   }
   cluster.sync();
-  uint32_t total = 0, before = 0;
-  for (int cc = 0; cc < C; ++cc) {
-    const uint32_t t = *cluster.map_shared_rank(&lps, cc);
-    total += t;
-    before += cc < c ? t : 0;
-  }
+  const uint32_t ptot = lane < C ? *cluster.map_shared_rank(&lps, lane) : 0;
+  const uint32_t total = __reduce_add_sync(0xffffffffu, ptot);
+  const uint32_t before = __reduce_add_sync(0xffffffffu, lane < c ? ptot : 0);
   const uint32_t target = (uint32_t)(((uint64_t)u * total) >> 20);
   if (total == 0) {                                           // a row whose every p rounds to 0
     if (c == 0 && tid == 0) a.sampled[r] = a.V - 1;
@@ -321,7 +342,10 @@ static cudaError_t launch_tree_verify(const VerArgs& a, cudaStream_t st) {
     cudaError_t e;
     // slices of a row over 8 CTAs, as few steps of 1024 logits as hold them
     const int per = (a.V + 8191) / 8192;
-    if (per <= 2) e = launch_sample_rows<2>(a, 8, st);
+    if (a.tnum >= (1ll << 31)) {
+      k_tree_sample_long<<<a.R, 1024, 0, st>>>(a);
+      e = cudaGetLastError();
+    } else if (per <= 2) e = launch_sample_rows<2>(a, 8, st);
     else if (per <= 8) e = launch_sample_rows<8>(a, 8, st);
     else if (per <= 20) e = launch_sample_rows<20>(a, 8, st);
     else if (per <= 40) e = launch_sample_rows<20>(a, 16, st);

@@ -80,8 +80,8 @@ EXB_DEV int k_shift(const exb_kv_view& kv, int head, int pg, int off) {
 
 // p = (e << 20) // sum for 0 <= e <= 2^24 by two multiplications: inv = ceil(2^86 / sum), and
 // e * (inv * sum - 2^86) < 2^24 * 2^42 = 2^66, so (e * inv) >> 66 is the exact quotient for
-// 2^24 <= sum < 2^42 (the row's largest term alone is 2^24; 2^18 positions).  Other sums: inv = 0, and
-// the division itself.
+// 2^24 <= sum < 2^42: the row's largest term alone is 2^24 (entry 0 of the table), and 2^18 terms stay
+// below 2^42.  Other sums: 0.
 EXB_DEV uint64_t prob_inverse(uint64_t sum) {
   if (sum < (1ull << 24) || sum >= (1ull << 42)) return 0;
   const uint64_t a = 1ull << 62;
@@ -95,11 +95,17 @@ EXB_DEV uint32_t prob_of(uint32_t e, uint64_t inv) {
   const uint64_t h = (uint64_t)e * (uint32_t)(inv >> 32) + (t >> 32);
   return (uint32_t)(h >> 34);
 }
-EXB_DEV uint32_t prob_slow(uint32_t e, uint64_t sum) { return sum ? (uint32_t)(((uint64_t)e << 20) / sum) : 0u; }
 
 // the table value at distance d, from a copy of the table in shared memory
 EXB_DEV uint32_t exp_sm(const int32_t* T, uint32_t d) {
   if (d >= (40u << 16)) return 0;
+  const int a = T[d >> 8], b = T[(d >> 8) + 1];
+  return (uint32_t)(a - (((a - b) * (int)(d & 255) + 128) >> 8));
+}
+
+// the same without a branch: entries 10240 and 10241 of the copy hold 0
+EXB_DEV uint32_t exp_sm_flat(const int32_t* T, uint32_t d) {
+  d = min(d, 40u << 16);
   const int a = T[d >> 8], b = T[(d >> 8) + 1];
   return (uint32_t)(a - (((a - b) * (int)(d & 255) + 128) >> 8));
 }
