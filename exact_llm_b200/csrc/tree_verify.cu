@@ -92,16 +92,16 @@ __global__ void __launch_bounds__(1024) k_tree_sample_long(const VerArgs a) { sa
 constexpr int TV_THREADS = 512;
 
 template <int IT>
-__global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(const VerArgs a, int slice) {
+__global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(const VerArgs a, int slice, int ahead) {
   extern __shared__ __align__(128) unsigned char sm[];
   int32_t* T = reinterpret_cast<int32_t*>(sm);
   constexpr int NW = TV_THREADS / 32;
   __shared__ int red[NW];
   __shared__ uint64_t red64[NW];
   __shared__ uint32_t seg[IT * NW];
-  __shared__ int lmax, lwide, lfirst;
+  __shared__ int lmax, lwide, lfirst, gmax, gwide;
   __shared__ uint64_t lsum, linv;
-  __shared__ uint32_t lps;
+  __shared__ uint32_t lps, gps[2];
   __shared__ uint64_t tbar;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), c = (int)cluster.block_rank();
@@ -129,7 +129,8 @@ __global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(con
     big |= (uint32_t)(hi ^ (lo >> 31)) | ((uint32_t)(wh + (1 << 14)) >> 15);
     return (int)__funnelshift_r((uint32_t)w, (uint32_t)wh, 16);
   };
-  constexpr int NB = IT < 4 ? IT : 4;                         // loads in flight a thread
+  constexpr int NB = IT < 4 ? IT : IT % 5 ? 4 : 5;            // loads in flight a thread
+  static_assert(IT % NB == 0, "whole batches");
 #pragma unroll
   for (int it0 = 0; it0 < IT; it0 += NB) {
     longlong2 v[NB];
@@ -155,6 +156,13 @@ __global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(con
       m = max(m, max(y[2 * (it0 + k)], y[2 * (it0 + k) + 1]));
     }
   }
+  // the same slice of the row that is read when this one is done: into L2 while the cluster confers
+  if (r + ahead < a.R) {
+    const char* p = reinterpret_cast<const char*>(row + (int64_t)ahead * a.ld);
+    const char* p0 = reinterpret_cast<const char*>((uintptr_t)p & ~(uintptr_t)15);
+    const int bytes = n * 8 & ~15;
+    for (int o = tid * 2048; o < bytes; o += TV_THREADS * 2048) prefetch_l2_bulk(p0 + o, min(2048, bytes - o));
+  }
   m = __reduce_max_sync(0xffffffffu, m);
   if (lane == 0) red[warp] = m;
   const int any_big = __syncthreads_or(big != 0);
@@ -163,10 +171,17 @@ __global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(con
     if (lane == 0) { lmax = m; lwide = any_big; }
   }
   cluster.sync();
-  // every warp reads all peers' words at once, one a lane
+  // one warp reads the peers' words, all at once, and leaves the result to the CTA: a word of another
+  // SM is dear (16 warps reading 8 peers took 0.9 us a time)
   const int peer = lane & (C - 1);
-  const int M = __reduce_max_sync(0xffffffffu, *cluster.map_shared_rank(&lmax, peer));
-  const bool wide = __any_sync(0xffffffffu, *cluster.map_shared_rank(&lwide, peer));
+  if (warp == 0) {
+    const int M0 = __reduce_max_sync(0xffffffffu, *cluster.map_shared_rank(&lmax, peer));
+    const bool w0 = __any_sync(0xffffffffu, *cluster.map_shared_rank(&lwide, peer));
+    if (lane == 0) { gmax = M0; gwide = w0; }
+  }
+  __syncthreads();
+  const int M = gmax;
+  const bool wide = gwide;
   if (wide) {
     if (u >= 0 && !mbar_wait(&tbar, 0)) return;               // no copy is left in flight
     if (c == 0) sample_row<TV_THREADS>(a, r);
@@ -243,36 +258,47 @@ __global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(con
     if (lane == 0) lps = t;
   }
   cluster.sync();
-  const uint32_t ptot = lane < C ? *cluster.map_shared_rank(&lps, lane) : 0;
-  const uint32_t total = __reduce_add_sync(0xffffffffu, ptot);
-  const uint32_t before = __reduce_add_sync(0xffffffffu, lane < c ? ptot : 0);
+  if (warp == 0) {
+    const uint32_t t = lane < C ? *cluster.map_shared_rank(&lps, lane) : 0;
+    const uint32_t t0 = __reduce_add_sync(0xffffffffu, t), t1 = __reduce_add_sync(0xffffffffu, lane < c ? t : 0);
+    if (lane == 0) { gps[0] = t0; gps[1] = t1; }
+  }
+  auto all_read = cluster.barrier_arrive();                  // this CTA reads no other's memory any more
+  __syncthreads();
+  const uint32_t total = gps[0], before = gps[1];
   const uint32_t target = (uint32_t)(((uint64_t)u * total) >> 20);
   if (total == 0) {                                           // a row whose every p rounds to 0
     if (c == 0 && tid == 0) a.sampled[r] = a.V - 1;
   } else if (before <= target && target < before + lps) {     // one CTA: its segment, then its lane
-    // each warp scans the segments in order, 32 at a time; the segment's own warp goes on
-    int k = 0;
-    uint32_t at = before;
-    for (int k0 = 0; k0 < IT * NW; k0 += 32) {
-      const uint32_t x = k0 + lane < IT * NW ? seg[k0 + lane] : 0;
-      uint32_t inc = x;
+    // every warp looks for the segment, a lane over NS neighbouring ones; the segment's own warp goes on
+    constexpr int NS = (IT * NW + 31) / 32;
+    uint32_t x[NS], mine = 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const uint32_t w = __shfl_up_sync(0xffffffffu, inc, o); inc += lane >= o ? w : 0; }
-      const unsigned hit = __ballot_sync(0xffffffffu, at + inc > target);
-      if (hit) {
-        const int l = __ffs(hit) - 1;
-        k = k0 + l;
-        at += __shfl_sync(0xffffffffu, inc - x, l);
-        break;
-      }
-      at += __shfl_sync(0xffffffffu, inc, 31);
+    for (int i = 0; i < NS; ++i) {
+      x[i] = lane * NS + i < IT * NW ? seg[lane * NS + i] : 0;
+      mine += x[i];
     }
+    uint32_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const uint32_t w = __shfl_up_sync(0xffffffffu, inc, o); inc += lane >= o ? w : 0; }
+    const int own = __ffs(__ballot_sync(0xffffffffu, before + inc > target)) - 1;
+    uint32_t at = before + inc - mine;
+    int k = lane * NS;
+#pragma unroll
+    for (int i = 0; i + 1 < NS; ++i)
+      if (k == lane * NS + i && at + x[i] <= target) { at += x[i]; ++k; }
+    k = __shfl_sync(0xffffffffu, k, own);
+    at = __shfl_sync(0xffffffffu, at, own);
     if (warp == k % NW) {
       uint32_t pa = 0, pb = 0;
 #pragma unroll
       for (int it = 0; it < IT; ++it)
-        if (it == k / NW) { pa = (uint32_t)y[2 * it]; pb = (uint32_t)y[2 * it + 1]; }
-      uint32_t inc = pa + pb;
+      {                                                       // masks: a select by index would put y in memory
+        const uint32_t is = 0u - (uint32_t)(it == k / NW);
+        pa |= (uint32_t)y[2 * it] & is;
+        pb |= (uint32_t)y[2 * it + 1] & is;
+      }
+      inc = pa + pb;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) { const uint32_t w = __shfl_up_sync(0xffffffffu, inc, o); inc += lane >= o ? w : 0; }
       const unsigned hit = __ballot_sync(0xffffffffu, at + inc > target);
@@ -282,7 +308,7 @@ __global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(con
       }
     }
   }
-  cluster.sync();                                             // the peers' words stay until they are read
+  cluster.barrier_wait(std::move(all_read));                 // this CTA's words stay until they are read
 }
 
 // One warp per sequence walks from node 0: 32 candidates at a time, the lowest one that fits.
@@ -334,7 +360,7 @@ static cudaError_t launch_sample_rows(const VerArgs& a, int C, cudaStream_t st) 
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_tree_sample<IT>, a, (a.V + 2 * C - 1) / (2 * C) * 2);
+  return cudaLaunchKernelEx(&cfg, k_tree_sample<IT>, a, (a.V + 2 * C - 1) / (2 * C) * 2, 2 * 148 / C);
 }
 
 static cudaError_t launch_tree_verify(const VerArgs& a, cudaStream_t st) {

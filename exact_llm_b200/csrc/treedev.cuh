@@ -84,11 +84,17 @@ EXB_DEV int k_shift(const exb_kv_view& kv, int head, int pg, int off) {
 // below 2^42.  Other sums: 0.
 EXB_DEV uint64_t prob_inverse(uint64_t sum) {
   if (sum < (1ull << 24) || sum >= (1ull << 42)) return 0;
-  const uint64_t a = 1ull << 62;
-  const uint64_t q0 = a / sum, r0 = a - q0 * sum;
-  const uint64_t q1 = (r0 << 12) / sum, r1 = (r0 << 12) - q1 * sum;
-  const uint64_t q2 = (r1 << 12) / sum, r2 = (r1 << 12) - q2 * sum;
-  return (q0 << 24) + (q1 << 12) + q2 + (r2 ? 1 : 0);
+  // a double's estimate is within 2^10 of the quotient (below 2^62 + 1), so the remainder 2^86 - q sum is
+  // below 2^53 and its low 64 bits are all of it; the second estimate is within one of the rest
+  const double rc = __drcp_rn((double)sum);
+  int64_t q = (int64_t)(rc * 77371252455336267181195264.0);             // 2^86
+  int64_t r = (int64_t)(0ull - (uint64_t)q * sum);
+  const int64_t dq = (int64_t)floor((double)r * rc);
+  q += dq;
+  r -= dq * (int64_t)sum;
+  while (r < 0) { r += (int64_t)sum; --q; }
+  while (r >= (int64_t)sum) { r -= (int64_t)sum; ++q; }
+  return (uint64_t)q + (r ? 1 : 0);
 }
 EXB_DEV uint32_t prob_of(uint32_t e, uint64_t inv) {
   const uint64_t t = (uint64_t)e * (uint32_t)inv;
