@@ -43,7 +43,7 @@ SIGNATURES = {
     "exb_linear_channel": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
-    "exb_tree_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 4),
+    "exb_tree_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 3),
     "exb_tree_attention": (ctypes.c_int, [ctypes.POINTER(KvView), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
                                           ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,

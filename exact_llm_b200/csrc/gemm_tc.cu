@@ -24,6 +24,7 @@
 #include "common.cuh"
 #include "exb_internal.h"
 #include "gemvdev.cuh"
+#include "tcdev.cuh"
 
 namespace exb {
 
@@ -31,7 +32,6 @@ constexpr int TC_BM = 128;                              // output rows per tile 
 constexpr int TC_PAD = TC_PAD_ROWS;                     // activation rows are padded to this
 constexpr int TC_STAGES = 4;
 constexpr int TC_A_BYTES = TC_BM * 128;                 // one group of 128 weight rows
-constexpr uint32_t TC_WAIT_LIMIT = 1u << 24;
 
 // Tile geometry for BN activation rows per tile (MMA N = 8, 64 or 128).  Every epilogue thread owns
 // one output row (TMEM lane) and CW activation columns; BN = 128 takes 16 epilogue warps (four per
@@ -75,66 +75,6 @@ struct TcArgs {
   unsigned long long* zero = nullptr; int nzero = 0;   // cleared by CTA (0, 0) for a later producer
 };
 
-// ---------------------------------------------------------------- PTX wrappers
-EXB_DEV bool tc_wait(uint64_t* bar, uint32_t parity) {
-  for (uint32_t i = 0; i < TC_WAIT_LIMIT; ++i)
-    if (mbar_try_wait(bar, parity)) return true;
-  return false;
-}
-EXB_DEV void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-      : "memory");
-}
-EXB_DEV void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-EXB_DEV void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-EXB_DEV void tc_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
-EXB_DEV void tc_mma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n"
-      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
-      : "memory");
-}
-// 8 consecutive 32-bit TMEM columns of this thread's lane
-EXB_DEV void tmem_ld8(uint32_t taddr, int32_t* v) {
-  uint32_t r[8];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr));
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (int32_t)r[i];
-}
-// 16 consecutive 32-bit TMEM columns of this thread's lane
-EXB_DEV void tmem_ld16(uint32_t taddr, int32_t* v) {
-  uint32_t r[16];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = (int32_t)r[i];
-}
-EXB_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// t + a * b with a 32 x 32 -> 64-bit product (one multiply-add; wraps modulo 2^64 like numpy)
-EXB_DEV int64_t mad_wide(int32_t a, int32_t b, int64_t t) {
-  int64_t d;
-  asm("mad.wide.s32 %0, %1, %2, %3;" : "=l"(d) : "r"(a), "r"(b), "l"(t));
-  return d;
-}
-
-// Shared-memory matrix descriptor: K-major operand in the 128-byte swizzled layout written by
-// TMA (rows of 128 bytes, 8-row core groups 1024 bytes apart), advanced by 32 bytes per K-step.
-EXB_DEV uint64_t tc_desc(const void* tile, int kstep) {
-  const uint32_t addr = smem_u32(tile) + 32u * (uint32_t)kstep;
-  return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
-         (2ull << 61);
-}
 // Instruction descriptor: int32 accumulate, A = signed int8 (weights), B = unsigned (low digit)
 // or signed (high digit) int8, both K-major, M = 128, N = BN.
 template <int BN>

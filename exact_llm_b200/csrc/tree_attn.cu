@@ -11,7 +11,7 @@
 #include <cmath>
 
 #include "exb_internal.h"
-#include "treedev.cuh"
+#include "tree_tc.h"
 
 namespace cg = cooperative_groups;
 
@@ -38,7 +38,7 @@ struct TreeGeo {
   static constexpr int KS = HD < 32 ? 1 : HD / 32;           // 32-dim steps of a score
   static constexpr int OUT = KP * NR * HD;                   // partial outputs (int64)
   // exp table, partial outputs, score rows, the V rows' places
-  static size_t smem(int ldk) { return 41024 + (size_t)OUT * 8 + (size_t)(NR + 1) * ldk * 4; }
+  static size_t smem(int ldk) { return 41024 + (size_t)OUT * 8 + (size_t)(NR + 2) * ldk * 4; }
 };
 // score row pitch for n positions: 4 mod 16 words, so a warp's stores and loads hit 32 banks
 inline int tree_pitch(int64_t n) { return (int)((n + 15) / 16 * 16 + 4); }
@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
   int32_t* T = reinterpret_cast<int32_t*>(sm);                               // exp table
   int64_t* pout = reinterpret_cast<int64_t*>(sm + 41024);                    // KP x NR x HD
   int32_t* sc = reinterpret_cast<int32_t*>(sm + 41024 + (size_t)G::OUT * 8); // NR x ldk
-  uint32_t* vat = reinterpret_cast<uint32_t*>(sc + (size_t)NR * ldk);        // V row of every position, in 16 bytes
+  int64_t* vat = reinterpret_cast<int64_t*>(sc + (size_t)NR * ldk);          // V row of every position, in elements
   __shared__ int64_t lmax[NR], lsum[NR];
   __shared__ int64_t wmax[8][NR];
   __shared__ uint64_t pinv[NR];
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
       if (store && tq == 0) {                                // V is needed after the exchanges: into L2 now
         const int32_t* vr = v_row(kv, j, max(pg, 0), off);
         if (pg >= 0) prefetch_l2_bulk(vr, HD * 4);
-        vat[t] = pg >= 0 ? (uint32_t)((vr - kv.v) >> 2) : 0u;        // a key that is not there has p = 0
+        vat[t] = pg >= 0 ? vr - kv.v : 0;       // a key that is not there has p = 0
       }
     }
   };
@@ -364,11 +364,11 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
     uint64_t inv[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) inv[nt] = pinv[nt * 8 + g];
-    const int4* vbase = reinterpret_cast<const int4*>(kv.v) + (dlive ? dg * 8 + g : 0);
+    const int32_t* vbase = kv.v + (dlive ? dg * 32 + 4 * g : 0);
     auto load_v = [&](int u, int4* v) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        v[i] = __ldg(vbase + vat[u + tq + 4 * i]);           // past the CTA's keys p is 0
+        v[i] = __ldg(reinterpret_cast<const int4*>(vbase + vat[u + tq + 4 * i]));           // past the CTA's keys p is 0
       }
     };
     int4 v[8];
@@ -452,86 +452,6 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
   cluster.sync();                                            // peers' shared memory stays until it is read
 }
 
-// ---------------------------------------------------------------- any size, slowly
-// One CTA per (row, head): the scores are computed anew in each of the three passes.
-constexpr int TS_THREADS = 128;
-
-__global__ void __launch_bounds__(TS_THREADS) k_tree_simple(const TreeArgs a) {
-  __shared__ int64_t red[TS_THREADS / 32];
-  __shared__ int64_t pt[TS_THREADS];
-  __shared__ const int32_t* vrow[TS_THREADS];
-  __shared__ int16_t qsm[128];
-  const int r = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-  const exb_kv_view& kv = a.kv;
-  const int hd = kv.hd, j = h / a.rep;
-  if (r == 0 && h == 0)                                // every sequence is looked over once
-    for (int i = tid; i < a.B; i += TS_THREADS) tree_seq(a, i, true);
-  int b = -1;
-  for (int i = 0; i < a.B; ++i)
-    if (r >= a.row_start[i] && r < a.row_start[i + 1]) { b = i; break; }
-  int64_t* out = a.out + ((size_t)r * a.H + h) * hd;
-  TreeSeq sq;
-  if (b >= 0) sq = tree_seq(a, b, false);
-  const uint64_t* mask = a.mask + (size_t)r * a.W;
-  const int32_t* row = a.table + (size_t)(b < 0 ? 0 : b) * a.MP;
-  const int qs = a.qs[(size_t)r * a.H + h];
-  if (tid < hd) qsm[tid] = a.q[((size_t)r * a.H + h) * hd + tid];
-  __syncthreads();
-  auto seen = [&](int t) { return t < sq.ctx || ((mask[(t - sq.ctx) >> 6] >> ((t - sq.ctx) & 63)) & 1); };
-  // score of position t; false where it is hidden
-  auto score = [&](int t, int64_t& s, int& pg, int& off) {
-    if (t >= sq.S || !seen(t)) return false;
-    pg = page_of(a, row, t, off);
-    if (pg < 0) return false;
-    const int16_t* k = kv.k + (int64_t)pg * kv.k_page + (int64_t)j * kv.k_head + (int64_t)off * kv.k_pos;
-    int64_t acc = 0;
-    for (int d = 0; d < hd; ++d) acc += (int)qsm[d] * (int)k[d];
-    const int ks = kv.ks[(int64_t)pg * kv.s_page + (int64_t)j * kv.s_head + (int64_t)off * kv.s_pos];
-    s = shr64((int64_t)((uint64_t)acc * (uint64_t)a.inv), 32 - qs - ks);
-    return true;
-  };
-  auto block_max = [&](int64_t v) {
-    for (int o = 16; o > 0; o >>= 1) { const int64_t w = __shfl_xor_sync(0xffffffffu, v, o); v = w > v ? w : v; }
-    __syncthreads();
-    if ((tid & 31) == 0) red[tid >> 5] = v;
-    __syncthreads();
-    for (int i = 0; i < TS_THREADS / 32; ++i) v = red[i] > v ? red[i] : v;
-    return v;
-  };
-  int64_t s;
-  int pg, off;
-  int64_t m = INT64_MIN;
-  for (int t = tid; t < sq.S; t += TS_THREADS)
-    if (score(t, s, pg, off)) m = s > m ? s : m;
-  m = block_max(m);
-  int64_t sum = 0;
-  for (int t = tid; t < sq.S; t += TS_THREADS)
-    if (score(t, s, pg, off)) sum += tree_exp(a.exp_t, (uint64_t)m - (uint64_t)s);
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  __syncthreads();
-  if ((tid & 31) == 0) red[tid >> 5] = sum;
-  __syncthreads();
-  sum = 0;
-  for (int i = 0; i < TS_THREADS / 32; ++i) sum += red[i];
-  uint64_t acc = 0;
-  for (int t0 = 0; t0 < sq.S; t0 += TS_THREADS) {
-    int64_t p = 0;
-    const int32_t* v = nullptr;
-    if (score(t0 + tid, s, pg, off)) {
-      p = (int64_t)(((uint64_t)tree_exp(a.exp_t, (uint64_t)m - (uint64_t)s) << 20) / (uint64_t)sum);
-      v = kv.v + (int64_t)pg * kv.v_page + (int64_t)j * kv.v_head + (int64_t)off * kv.v_pos;
-    }
-    __syncthreads();
-    pt[tid] = p;
-    vrow[tid] = v;
-    __syncthreads();
-    if (tid < hd)
-      for (int t = 0; t < TS_THREADS; ++t)
-        if (pt[t]) acc += (uint64_t)pt[t] * (uint64_t)(int64_t)vrow[t][tid];
-  }
-  if (tid < hd) out[tid] = shr64((int64_t)acc, 20);
-}
-
 template <int HD, int NT>
 static cudaError_t launch_cluster(const TreeArgs& a, int C, int ldk, cudaStream_t st) {
   using G = TreeGeo<HD, NT>;
@@ -566,29 +486,27 @@ static cudaError_t launch_cluster_hd(const TreeArgs& a, int C, int ldk, cudaStre
   }
 }
 
-// elements from the first V row of a layer to behind its last
-static int64_t v_extent(const exb_kv_view& kv) {
-  return (kv.pages - 1) * std::abs(kv.v_page) + (kv.KV - 1) * std::abs(kv.v_head) + (kv.page - 1) * std::abs(kv.v_pos) + kv.hd;
+// Many rows in a group and much work: the tensor-core kernels.
+static bool use_tc(const TreeArgs& a) {
+  return (int64_t)a.R * a.rep >= 32ll * a.B && (int64_t)a.R * a.H * a.cap >= (1ll << 22);
 }
 
-static cudaError_t launch_tree_attention(const TreeArgs& a, cudaStream_t st) {
+static cudaError_t launch_tree_attention(const TreeArgs& a, void* workspace, cudaStream_t st) {
   // rows per tile: 16 where the trees have that many in a group
   const int NT = (int64_t)a.R * a.rep > 8ll * a.B ? 2 : 1, NR = 8 * NT;
   // CTAs per cluster: as many as keep every cluster resident at once (two CTAs an SM, one with 16 rows
   // or a long score array), each with 64 positions at least; more where the scores need the room
   const int64_t clusters = std::max<int64_t>(a.B, ((int64_t)a.R * a.rep + NR - 1) / NR) * a.kv.KV;
   auto pitch = [&](int c) { return tree_pitch(((a.cap + c - 1) / c + 31) / 16 * 16); };
-  auto smem_of = [&](int c) { return 41024 + (size_t)2048 * NR + (size_t)(NR + 1) * pitch(c) * 4; };
+  auto smem_of = [&](int c) { return 41024 + (size_t)2048 * NR + (size_t)(NR + 2) * pitch(c) * 4; };
   int C = 1;
   while (C < 16 && (smem_of(C) > (size_t)TREE_SMEM_MAX ||
                     ((int64_t)C * 64 < a.cap && clusters * 2 * C <= (NT == 2 || smem_of(2 * C) > 110 * 1024 ? 148 : 296))))
     C *= 2;
   const size_t smem = smem_of(C);
   const int ldk = pitch(C);
-  if (smem <= (size_t)TREE_SMEM_MAX && v_extent(a.kv) < (1ll << 34))       // V places: 32 bits of 16 bytes
-    return NT == 2 ? launch_cluster_hd<2>(a, C, ldk, st) : launch_cluster_hd<1>(a, C, ldk, st);
-  k_tree_simple<<<dim3(a.R, a.H), TS_THREADS, 0, st>>>(a);
-  return cudaGetLastError();
+  if (smem > (size_t)TREE_SMEM_MAX || use_tc(a)) return launch_tree_tc(a, workspace, st);
+  return NT == 2 ? launch_cluster_hd<2>(a, C, ldk, st) : launch_cluster_hd<1>(a, C, ldk, st);
 }
 
 // what is wrong with a cache description, or nullptr
@@ -614,9 +532,8 @@ using namespace exb;
 
 extern "C" {
 
-size_t exb_tree_attention_workspace_bytes(int R, int H, int KV, int hd) {
-  (void)R; (void)H; (void)KV; (void)hd;
-  return 256;
+size_t exb_tree_attention_workspace_bytes(int R, int H, int B) {
+  return R < 1 || H < 1 || B < 0 ? 0 : tt_workspace_bytes(R, H, B);
 }
 
 int exb_tree_attention(const exb_kv_view* kv, const int16_t* q, const int32_t* qs, int R, int H, const int32_t* table,
@@ -632,14 +549,14 @@ int exb_tree_attention(const exb_kv_view* kv, const int16_t* q, const int32_t* q
   if (mask_words < 1 || mask_words > 64 || max_pages < 1) TREE_FAIL(EXB_EINVAL, "exb_tree_attention: 1 <= mask_words <= 64 and max_pages >= 1");
   if ((int64_t)max_pages * kv->page >= (1ll << 30)) TREE_FAIL(EXB_EINVAL, "exb_tree_attention: a table row names 2^30 positions or more");
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)exp_t | (uintptr_t)workspace) & 15) TREE_FAIL(EXB_EINVAL, "exb_tree_attention: q, exp_t, out and workspace must be 16-byte aligned");
-  if (!workspace || workspace_bytes < exb_tree_attention_workspace_bytes(R, H, kv->KV, kv->hd))
+  if (!workspace || workspace_bytes < exb_tree_attention_workspace_bytes(R, H, B))
     TREE_FAIL(EXB_EINVAL, "exb_tree_attention: workspace too small");
   TreeArgs a;
   a.kv = *kv; a.q = q; a.qs = qs; a.table = table; a.ctx = ctx; a.row_start = row_start; a.mask = mask;
   a.exp_t = exp_t; a.out = out; a.status = status; a.R = R; a.H = H; a.rep = H / kv->KV; a.B = B; a.MP = max_pages;
   a.W = mask_words; a.cap = (int64_t)max_pages * kv->page; a.page_div = fast_div(kv->page);
   a.inv = (int64_t)std::nearbyint(65536.0 / std::sqrt((double)kv->hd));
-  const cudaError_t e = B ? launch_tree_attention(a, (cudaStream_t)stream)
+  const cudaError_t e = B ? launch_tree_attention(a, workspace, (cudaStream_t)stream)
                           : cudaMemsetAsync(out, 0, (size_t)R * H * kv->hd * 8, (cudaStream_t)stream);
   if (e != cudaSuccess) TREE_FAIL(EXB_ECUDA, std::string("exb_tree_attention: ") + cudaGetErrorString(e));
   return EXB_OK;

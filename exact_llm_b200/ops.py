@@ -203,7 +203,7 @@ def _tree_attention(q, qs, k, ks, v, table, ctx, row_start, mask, exp_t, status=
     out = torch.empty((R, H, hd), dtype=torch.int64, device=q.device)
     if R == 0:
         return out
-    nb = lib.exb_tree_attention_workspace_bytes(R, H, k.shape[1], hd)
+    nb = lib.exb_tree_attention_workspace_bytes(R, H, B)
     ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
     with _on(q.device) as stream:
         check(lib.exb_tree_attention(kv, q.data_ptr(), qs.data_ptr(), R, H, table.data_ptr(), B, table.shape[1],

@@ -116,8 +116,10 @@ typedef struct exb_kv_view {
  * i % 64 of mask[row][i / 64] is set; a row that sees nothing gives zeros.
  *   q int16 (R, H, hd), qs int32 (R, H) shifts (0..63); layer 0 of kv is used; H % KV == 0
  *   table int32 (B, max_pages), ctx int32 (B), row_start int32 (B+1), mask (R, mask_words)
- *   exp_t int32 (10242) the Q24 table; out int64 (R, H, hd) */
-size_t exb_tree_attention_workspace_bytes(int R, int H, int KV, int hd);
+ *   exp_t int32 (10242) the program's Q24 table (entry 0 is 2^24); out int64 (R, H, hd)
+ *   workspace: exb_tree_attention_workspace_bytes(R, H, B) device bytes
+ * q, out, exp_t and workspace 16-byte aligned. */
+size_t exb_tree_attention_workspace_bytes(int R, int H, int B);
 int exb_tree_attention(const exb_kv_view* kv, const int16_t* q, const int32_t* qs, int R, int H, const int32_t* table,
                        int B, int max_pages, const int32_t* ctx, const int32_t* row_start, const uint64_t* mask,
                        int mask_words, const int32_t* exp_t, int64_t* out, void* workspace, size_t workspace_bytes,

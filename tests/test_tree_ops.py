@@ -33,8 +33,12 @@ def exp_t(gpu):
 ORDER = ("q", "qs", "k", "ks", "v", "table", "ctx", "row_start", "mask")
 
 
-def _attend(torch, exp_t, p, status=None, **replace):
+def _attend(torch, exp_t, p, status=None, wide=False, **replace):
     a = {n: _dev(torch, p[n]) for n in ORDER}
+    if wide:                                                # unused columns: room for 2^20 positions
+        page = p["k"].shape[2]
+        more = -(-(1 << 20) // page) - p["table"].shape[1]
+        a["table"] = torch.nn.functional.pad(a["table"], (0, more), value=-1).contiguous()
     a.update(replace)
     return torch.ops.exact.tree_attention(*[a[n] for n in ORDER], exp_t, status)
 
@@ -164,20 +168,26 @@ ATTENTION = {
 }
 
 
+# A table with room for a long cache takes the kernels for long caches, whatever the lengths in it are.
+WIDE = pytest.mark.parametrize("wide", [False, True], ids=["", "long table"])
+
+
 @pytest.mark.gpu
+@WIDE
 @pytest.mark.parametrize("name", list(ATTENTION))
-def test_attention(gpu, exp_t, name):
+def test_attention(gpu, exp_t, name, wide):
     p = ref.problem(len(name), **ATTENTION[name])
     status = gpu.zeros(1, dtype=gpu.int32, device="cuda")
-    got = _attend(gpu, exp_t, p, status).cpu().numpy()
+    got = _attend(gpu, exp_t, p, status, wide).cpu().numpy()
     assert np.array_equal(got, ref.attention(**p))
     assert int(status) == 0
 
 
 @pytest.mark.gpu
+@WIDE
 @pytest.mark.parametrize("hd", [16, 32, 64, 128])
 @pytest.mark.parametrize("nodes", [1, 3, 40])
-def test_attention_extreme_values(gpu, exp_t, hd, nodes):
+def test_attention_extreme_values(gpu, exp_t, hd, nodes, wide):
     """Every factor at the end of its type: sums and digits at their largest."""
     for seed, (qv, kv, vv) in enumerate([(32767, 32767, 2**31 - 1), (-32768, 32767, -2**31), (-32768, -32768, -1),
                                          (255, -256, 2**23), (-1, 1, -2**23 - 1)]):
@@ -189,23 +199,25 @@ def test_attention_extreme_values(gpu, exp_t, hd, nodes):
         p["v"][:] = vv
         p["v"][:, :, 1::3] = -1 - vv
         p["qs"][:], p["ks"][:] = 0, 0
-        assert np.array_equal(_attend(gpu, exp_t, p).cpu().numpy(), ref.attention(**p)), seed
+        assert np.array_equal(_attend(gpu, exp_t, p, None, wide).cpu().numpy(), ref.attention(**p)), seed
 
 
 @pytest.mark.gpu
+@WIDE
 @pytest.mark.parametrize("seed", range(12))
-def test_attention_random(gpu, exp_t, seed):
+def test_attention_random(gpu, exp_t, seed, wide):
     rng = np.random.default_rng(1000 + seed)
     KV, rep, hd = int(rng.integers(1, 5)), int(rng.integers(1, 9)), int(rng.choice([16, 32, 64, 128]))
     B = int(rng.integers(1, 6))
     ctx = [int(x) for x in np.exp(rng.uniform(0, 7, B)).astype(int) - 1]
     nodes = [int(x) for x in np.exp(rng.uniform(0, 4.3, B)).astype(int)]
     p = ref.problem(seed, H=KV * rep, KV=KV, hd=hd, page=int(rng.choice([1, 7, 16, 64, 100])), ctx=ctx, nodes=nodes)
-    assert np.array_equal(_attend(gpu, exp_t, p).cpu().numpy(), ref.attention(**p))
+    assert np.array_equal(_attend(gpu, exp_t, p, None, wide).cpu().numpy(), ref.attention(**p))
 
 
 @pytest.mark.gpu
-def test_attention_masks(gpu, exp_t):
+@WIDE
+def test_attention_masks(gpu, exp_t, wide):
     """Rows that see nothing give zeros; bits past the tree count for nothing; any set of nodes will do."""
     p = ref.problem(5, H=6, KV=2, hd=64, page=16, ctx=[0, 20], nodes=[9, 70], words=3)
     rng = np.random.default_rng(0)
@@ -213,13 +225,14 @@ def test_attention_masks(gpu, exp_t):
     p["mask"][2] = 0                                        # no context, no node
     p["mask"][5] = np.int64(-1) << np.int64(9)              # only bits past the tree
     p["mask"][12] = 0                                       # the context alone
-    got = _attend(gpu, exp_t, p).cpu().numpy()
+    got = _attend(gpu, exp_t, p, None, wide).cpu().numpy()
     assert np.array_equal(got, ref.attention(**p))
     assert not got[2].any() and not got[5].any() and got[12].any()
 
 
 @pytest.mark.gpu
-def test_attention_ignores_stale_rows(gpu, exp_t):
+@WIDE
+def test_attention_ignores_stale_rows(gpu, exp_t, wide):
     """Positions past the tree, other pages and hidden nodes hold anything: no bit changes."""
     p = ref.problem(6, H=14, KV=2, hd=64, page=32, ctx=[50, 200], nodes=[5, 40])
     want = ref.attention(**p)
@@ -229,11 +242,12 @@ def test_attention_ignores_stale_rows(gpu, exp_t):
         used[p["table"][b][pos // 32], :, pos % 32] = True
     for n, x in (("k", -32768), ("ks", 127), ("v", -2**31)):
         p[n][~used] = x
-    assert np.array_equal(_attend(gpu, exp_t, p).cpu().numpy(), want)
+    assert np.array_equal(_attend(gpu, exp_t, p, None, wide).cpu().numpy(), want)
 
 
 @pytest.mark.gpu
-def test_attention_strides(gpu, exp_t):
+@WIDE
+def test_attention_strides(gpu, exp_t, wide):
     """A layer of a slot cache, head-last storage, padded rows: the same bits, and the rows of other layers unread."""
     torch = gpu
     p = ref.problem(7, H=10, KV=2, hd=64, page=48, ctx=[100, 30], nodes=[7, 20])
@@ -250,11 +264,12 @@ def test_attention_strides(gpu, exp_t):
                 pad = torch.full((*x.shape[:-1], x.shape[-1] + 8), -7, dtype=x.dtype, device="cuda")
                 pad[..., :x.shape[-1]] = x
                 new[n] = pad[..., :x.shape[-1]]
-        assert np.array_equal(_attend(torch, exp_t, p, **new).cpu().numpy(), want), how
+        assert np.array_equal(_attend(torch, exp_t, p, None, wide, **new).cpu().numpy(), want), how
 
 
 @pytest.mark.gpu
-def test_attention_out_of_range(gpu, exp_t):
+@WIDE
+def test_attention_out_of_range(gpu, exp_t, wide):
     """A page id or a position that does not exist is left out and reported, never read."""
     torch = gpu
     p = ref.problem(8, H=4, KV=2, hd=32, page=16, ctx=[40], nodes=[6])
@@ -262,7 +277,7 @@ def test_attention_out_of_range(gpu, exp_t):
         x = dict(p, table=p["table"].copy())
         x["table"][0, 1] = bad                              # positions 16..31 are gone
         status = torch.zeros(1, dtype=torch.int32, device="cuda")
-        got = _attend(torch, exp_t, x, status).cpu().numpy()
+        got = _attend(torch, exp_t, x, status, wide).cpu().numpy()
         assert int(status) == 8
         keep = np.r_[0:16, 32:46]
         y = dict(p, table=np.array([[0, 1]], np.int32), ctx=np.array([24], np.int32))
@@ -272,13 +287,13 @@ def test_attention_out_of_range(gpu, exp_t):
             y[n] = np.ascontiguousarray(rows.reshape(2, 16, *rows.shape[1:]).swapaxes(1, 2))
         assert np.array_equal(got, ref.attention(**y))
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
-    _attend(torch, exp_t, dict(p, ctx=np.array([43], np.int32)), status)        # a node past the table's end
+    _attend(torch, exp_t, dict(p, ctx=np.array([43], np.int32)), status, wide)  # a node past the table's end
     assert int(status) == 8
     for rs in ([0, 7], [-1, 6], [4, 2]):
         status.zero_()
-        got = _attend(torch, exp_t, dict(p, row_start=np.array(rs, np.int32)), status)
+        got = _attend(torch, exp_t, dict(p, row_start=np.array(rs, np.int32)), status, wide)
         assert int(status) == 8 and not got.any()
-    got = _attend(torch, exp_t, dict(p, row_start=np.array([2, 5], np.int32)))   # rows that no sequence owns
+    got = _attend(torch, exp_t, dict(p, row_start=np.array([2, 5], np.int32)), None, wide)   # rows that no sequence owns
     assert not got[:2].any() and not got[5:].any() and got[2:5].any()
 
 
