@@ -5,8 +5,8 @@ reference's model/engine API (``model.ExactModel``) and its operator API (``impo
 exact_llm_b200.ops`` registers ``torch.ops.exact.gemv``).  All arithmetic runs in the CUDA library;
 there is no CPU fallback.
 """
-from . import configs, tables  # noqa: F401
+from . import configs, drafting, tables  # noqa: F401
 from ._lib import ExbError, lib  # noqa: F401
 from .model import Cache, ExactModel  # noqa: F401
 
-__all__ = ["ExactModel", "Cache", "ExbError", "configs", "tables", "lib"]
+__all__ = ["ExactModel", "Cache", "ExbError", "configs", "drafting", "tables", "lib"]

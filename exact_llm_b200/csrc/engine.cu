@@ -176,6 +176,10 @@ struct exb_model {
   int32_t *p_xs = nullptr, *p_qs = nullptr, *p_next = nullptr;
   void* p_dig = nullptr;
   unsigned long long* p_amax = nullptr;     // per-row max |h| published by the gate|up GEMM
+  // drafted trees (exb_tree_step): index arrays and the attention workspace, allocated on first use
+  char* t_arena = nullptr;
+  char* t_host = nullptr;                   // pinned staging of the index arrays, then of the results
+  size_t t_ws = 0, t_ws_bytes = 0;          // attention workspace: offset in t_arena, size
   // persistent decode-step kernel (step.cu): per-layer descriptors and accumulators
   bool tc_on = true;                    // multi-row chunks on the tensor-core GEMM
   bool tail_norm = false;               // decode: the o and down GEMVs finish the next norm in their last CTA
@@ -1154,6 +1158,8 @@ void exb_model_destroy(exb_model* m) {
   if (m->comm && nccl()) nccl()->comm_destroy(m->comm);
   cudaFree(m->p_arena);
   if (m->p_hrows) cudaFreeHost(m->p_hrows);
+  cudaFree(m->t_arena);
+  if (m->t_host) cudaFreeHost(m->t_host);
   if (m->h_ids) cudaFreeHost(m->h_ids);
   if (m->st) cudaStreamDestroy(m->st);
   delete m;
@@ -1496,8 +1502,30 @@ static int prefill_alloc(exb_model* m) {
   return EXB_OK;
 }
 
-// one chunk of R rows (R <= PCH): host ids / seq / pos already in m->p_hrows
-static int prefill_chunk(exb_model* m, int R, int64_t* logits_host, int32_t* next_host) {
+// the cache of every layer as a paged one: a slot is a page of max_seq positions
+static exb_kv_view kv_view_of(const exb_model* m) {
+  const exb_config& c = m->c;
+  exb_kv_view v = {};
+  v.k = m->kc; v.ks = m->ks; v.v = m->vc;
+  v.layers = c.NL; v.pages = c.max_batch; v.KV = c.KV; v.page = c.max_seq; v.hd = c.hd;
+  v.k_pos = v.v_pos = c.hd;
+  v.k_head = v.v_head = (int64_t)c.max_seq * c.hd;
+  v.k_page = v.v_page = v.k_head * c.KV;
+  v.k_layer = v.v_layer = (int64_t)m->kv_layer_elems;
+  v.s_pos = 1; v.s_head = c.max_seq; v.s_page = (int64_t)c.max_seq * c.KV; v.s_layer = v.s_page * c.max_batch;
+  return v;
+}
+
+// device arrays of a chunk whose rows are nodes of drafted trees
+struct TreeRows {
+  int B = 0, W = 0;
+  const int32_t *at = nullptr, *table = nullptr, *ctx = nullptr, *row_start = nullptr;
+  const uint64_t* mask = nullptr;
+};
+
+// one chunk of R rows (R <= PCH): host ids / seq / pos already in m->p_hrows.  With `tree` the rows
+// attend along their trees, every row's logits stay in m->p_raw and the call does not wait.
+static int prefill_chunk(exb_model* m, int R, int64_t* logits_host, int32_t* next_host, const TreeRows* tree = nullptr) {
   const exb_config& c = m->c;
   cudaStream_t st = m->st;
   const int D = c.D, Hd = c.H * c.hd, I = c.I;
@@ -1513,6 +1541,7 @@ static int prefill_chunk(exb_model* m, int R, int64_t* logits_host, int32_t* nex
   aa.out = m->p_ao; aa.ldo = Hd; aa.R = R; aa.H = c.H; aa.KV = c.KV; aa.hd = c.hd; aa.Smax = c.max_seq;
   aa.Tmax = c.rope_len; aa.err = m->err;
   aa.inv = (int64_t)std::nearbyint(65536.0 / std::sqrt((double)c.hd));
+  if (tree) aa.row_at = tree->at;
   // a chunk of consecutive positions of one sequence takes the query-tile attention kernel
   bool one_seq = m->attn_prefill;
   for (int r = 1; r < R && one_seq; ++r)
@@ -1542,7 +1571,15 @@ static int prefill_chunk(exb_model* m, int R, int64_t* logits_host, int32_t* nex
     CK(launch_norm_q(m->p_x, D, Ld.g1, R, D, m->p_xq, D, m->p_xs, st, false, dig, nullptr, 0, Tpad));
     CK(lin(m->p_xq, D, Ld.qkv, EPI_STORE, m->p_qkv, m->Nqkv));
     CK(launch_rope_cache(aa, st, false));
-    if (one_seq) CK(launch_attn_prefill(aa, st));       // query tiles share the cached K/V rows
+    if (tree) {
+      exb_kv_view kv = kv_view_of(m);
+      kv.layers = 1;
+      kv.k = aa.kc; kv.ks = aa.ks; kv.v = aa.vc;
+      const int rc = exb_tree_attention(&kv, aa.qq, aa.qs, R, c.H, tree->table, tree->B, 1, tree->ctx, tree->row_start,
+                                        tree->mask, tree->W, m->exp_t, aa.out, m->t_arena + m->t_ws, m->t_ws_bytes,
+                                        m->err, st);
+      if (rc) return rc;
+    } else if (one_seq) CK(launch_attn_prefill(aa, st));       // query tiles share the cached K/V rows
     else CK(launch_attn_decode(aa, st, false));
     CK(launch_quant(m->p_ao, Hd, R, Hd, m->p_xq, Hd, m->p_xs, st, false, dig, Tpad));
     CK(lin(m->p_xq, Hd, Ld.o, EPI_RESID, m->p_x, D));
@@ -1566,11 +1603,11 @@ static int prefill_chunk(exb_model* m, int R, int64_t* logits_host, int32_t* nex
   CK(launch_norm_q(m->p_x, D, m->gf, R, D, m->p_xq, D, m->p_xs, st, false, dig, nullptr, 0, Tpad));
   // head: unscaled per-group sums on the tensor cores, then the per-channel requant + argmax per row
   CK(lin(m->p_xq, D, m->head, EPI_RAW, m->p_raw, c.V));
-  int64_t* lg = logits_host ? m->p_raw : nullptr;             // requant in place (row by row, read before write)
+  int64_t* lg = logits_host || tree ? m->p_raw : nullptr;     // requant in place (row by row, read before write)
   CK(launch_head_rows(m->p_raw, c.V, R, m->head, m->p_xs, lg, c.V, m->p_next, st));
   if (logits_host) CK(cudaMemcpyAsync(logits_host, m->p_raw, sizeof(int64_t) * R * c.V, cudaMemcpyDeviceToHost, st));
   if (next_host) CK(cudaMemcpyAsync(next_host, m->p_next, sizeof(int32_t) * R, cudaMemcpyDeviceToHost, st));
-  CK(cudaStreamSynchronize(st));
+  if (!tree) CK(cudaStreamSynchronize(st));
   return EXB_OK;
 }
 
@@ -1660,6 +1697,129 @@ int exb_forward(exb_model* m, int n, const int32_t* ids, const int32_t* seqs, in
   }
   m->seq_len = len;
   return check_device_errors(m);
+}
+
+// ------------------------------------------------------------------------------------------ drafted trees
+static constexpr int TREE_WORDS = PCH / 64;
+
+// One step of every given sequence on a tree of drafted tokens: all nodes as one chunk, the target's
+// choice at each, the accepted path's cache rows moved together, the sequences advanced.
+int exb_tree_step(exb_model* m, int B, const int32_t* seqs, const int32_t* row_start, const int32_t* ids,
+                  const int32_t* parent, const int32_t* u20, int64_t tnum, int max_len, int32_t* n, int32_t* path,
+                  int32_t* tokens, int32_t* sampled, int64_t* logits) {
+  if (!m || !m->finalized) FAIL(EXB_EINVAL, "model not finalized");
+  const exb_config& c = m->c;
+  if (!prefill_tc_ok(m) || m->commit_on)
+    FAIL(EXB_EINVAL, "exb_tree_step: needs the tensor-core path (one GPU, a vocabulary of whole 128s, no trace, "
+                     "commitment or Freivalds capture)");
+  if (c.hd != 16 && c.hd != 32 && c.hd != 64 && c.hd != 128) FAIL(EXB_EINVAL, "exb_tree_step: hd must be 16, 32, 64 or 128");
+  if (B < 1 || B > c.max_batch || !seqs || !row_start || !ids || !parent || !n || !path || !tokens)
+    FAIL(EXB_EINVAL, "exb_tree_step: 1 <= B <= max_batch and no null argument");
+  const int R = row_start[B];
+  if (row_start[0] != 0 || R < 1 || R > chunk_rows(m)) FAIL(EXB_EINVAL, "exb_tree_step: 1 to 512 rows (256 for MoE) from row_start[0] = 0");
+  if (max_len < 1 || max_len > PCH) FAIL(EXB_EINVAL, "exb_tree_step: 1 <= max_len <= 512");
+  if (tnum < 1 || tnum > (1ll << 32)) FAIL(EXB_EINVAL, "exb_tree_step: temperature multiplier in [1, 2^32]");
+  std::vector<char> taken(c.max_batch, 0);
+  std::vector<int> depth(R);
+  std::vector<uint64_t> mask((size_t)R * TREE_WORDS, 0);
+  int most = 0;
+  for (int b = 0; b < B; ++b) {
+    const int r0 = row_start[b], T = row_start[b + 1] - r0, s = seqs[b];
+    if (T < 1) FAIL(EXB_EINVAL, "exb_tree_step: every sequence has at least its last token as node 0");
+    if (s < 0 || s >= c.max_batch || taken[s]) FAIL(EXB_EINVAL, "exb_tree_step: bad or repeated sequence slot");
+    taken[s] = 1;
+    if (m->seq_len[s] + T > c.max_seq) FAIL(EXB_EINVAL, "exb_tree_step: sequence longer than max_seq");
+    most = std::max(most, T);
+    for (int i = 0; i < T; ++i) {
+      const int p = parent[r0 + i];
+      if (i == 0 ? p != -1 : (p < 0 || p >= i)) FAIL(EXB_EINVAL, "exb_tree_step: node 0 has parent -1, every other an earlier node");
+      if (ids[r0 + i] < 0 || ids[r0 + i] >= c.V) FAIL(EXB_EINVAL, "exb_tree_step: token id out of range");
+      if (u20 && (u20[r0 + i] < -1 || u20[r0 + i] >= (1 << 20))) FAIL(EXB_EINVAL, "exb_tree_step: u20 outside [-1, 2^20)");
+      depth[r0 + i] = i ? depth[r0 + p] + 1 : 0;
+      uint64_t* w = mask.data() + (size_t)(r0 + i) * TREE_WORDS;
+      if (i)
+        for (int k = 0; k < TREE_WORDS; ++k) w[k] = mask[(size_t)(r0 + p) * TREE_WORDS + k];
+      w[i >> 6] |= 1ull << (i & 63);
+    }
+  }
+  int rc = prefill_alloc(m);
+  if (rc) return rc;
+  // index arrays in one block, results in another: one copy each way
+  const size_t nb = ((size_t)c.max_batch + 2) * 4, nr = (size_t)PCH * 4, np = (size_t)c.max_batch * PCH * 4;
+  size_t off = 0;
+  auto take = [&](size_t bytes) { const size_t o = off; off = (off + bytes + 255) & ~size_t(255); return o; };
+  const size_t o_mask = take((size_t)PCH * TREE_WORDS * 8), o_at = take(nr), o_par = take(nr), o_u = take(nr), o_tab = take(nb),
+               o_ctx = take(nb), o_rs = take(nb), in_bytes = off, o_n = take(nb), o_samp = take(nr), o_path = take(np),
+               o_tok = take(np), o_new = take(nb), all_bytes = off;
+  if (!m->t_arena) {
+    m->t_ws = all_bytes;
+    m->t_ws_bytes = exb_tree_attention_workspace_bytes(PCH, c.H, c.max_batch);
+    CK(cudaMallocHost(&m->t_host, all_bytes));
+    CK(cudaMalloc(&m->t_arena, all_bytes + m->t_ws_bytes));
+  }
+  char *h = m->t_host, *d = m->t_arena;
+  for (int r = 0, b = 0; r < R; ++r) {
+    while (r >= row_start[b + 1]) ++b;
+    m->p_hrows[r] = ids[r];
+    m->p_hrows[PCH + r] = seqs[b];
+    m->p_hrows[2 * PCH + r] = m->seq_len[seqs[b]] + depth[r];
+    reinterpret_cast<int32_t*>(h + o_at)[r] = m->seq_len[seqs[b]] + r - row_start[b];
+    reinterpret_cast<int32_t*>(h + o_u)[r] = u20 ? u20[r] : -1;
+  }
+  const int W = (most + 63) / 64;
+  for (int r = 0; r < R; ++r)
+    memcpy(h + o_mask + (size_t)r * W * 8, mask.data() + (size_t)r * TREE_WORDS, (size_t)W * 8);
+  memcpy(h + o_par, parent, (size_t)R * 4);
+  memcpy(h + o_tab, seqs, (size_t)B * 4);
+  memcpy(h + o_rs, row_start, (size_t)(B + 1) * 4);
+  for (int b = 0; b < B; ++b) reinterpret_cast<int32_t*>(h + o_ctx)[b] = m->seq_len[seqs[b]];
+  CK(cudaMemsetAsync(m->err, 0, sizeof(int), m->st));
+  CK(cudaMemcpyAsync(d, h, in_bytes, cudaMemcpyHostToDevice, m->st));
+  m->sel_rows = c.n_experts ? std::min(R, SEL_CAP) : 0;
+  auto i32 = [&](size_t o) { return reinterpret_cast<int32_t*>(d + o); };
+  TreeRows t;
+  t.B = B; t.W = W; t.at = i32(o_at); t.table = i32(o_tab); t.ctx = i32(o_ctx); t.row_start = i32(o_rs);
+  t.mask = reinterpret_cast<const uint64_t*>(d + o_mask);
+  g_hist_row0 = c.n_experts ? 0 : -1;
+  rc = prefill_chunk(m, R, logits, nullptr, &t);
+  g_hist_row0 = -1;
+  if (rc) return rc;
+  rc = exb_tree_verify(m->p_raw, c.V, R, c.V, i32(o_u), tnum, m->p_rows, i32(o_par), t.row_start, B, max_len, m->exp_t,
+                       i32(o_samp), i32(o_n), i32(o_path), i32(o_tok), m->st);
+  if (rc) return rc;
+  const exb_kv_view kv = kv_view_of(m);
+  rc = exb_kv_compact(&kv, t.table, B, 1, t.ctx, i32(o_path), max_len, i32(o_n), i32(o_new), m->err, m->st);
+  if (rc) return rc;
+  CK(cudaMemcpyAsync(h + in_bytes, d + in_bytes, o_tok + (size_t)B * max_len * 4 - in_bytes, cudaMemcpyDeviceToHost, m->st));
+  rc = check_device_errors(m);                               // waits for the stream
+  if (rc) return rc;
+  memcpy(n, h + o_n, (size_t)B * 4);
+  memcpy(path, h + o_path, (size_t)B * max_len * 4);
+  memcpy(tokens, h + o_tok, (size_t)B * max_len * 4);
+  if (sampled) memcpy(sampled, h + o_samp, (size_t)R * 4);
+  for (int b = 0; b < B; ++b) m->seq_len[seqs[b]] += n[b];
+  return EXB_OK;
+}
+
+int exb_seq_fork(exb_model* m, int src, int dst, int n) {
+  if (!m || !m->finalized) FAIL(EXB_EINVAL, "model not finalized");
+  const exb_config& c = m->c;
+  if (src < 0 || src >= c.max_batch || dst < 0 || dst >= c.max_batch || src == dst)
+    FAIL(EXB_EINVAL, "exb_seq_fork: two different sequence slots");
+  if (n < 0 || n > m->seq_len[src]) FAIL(EXB_EINVAL, "exb_seq_fork: the source holds fewer positions");
+  if (n) {
+    const int32_t h[3] = {src, dst, n};
+    int32_t* d = nullptr;
+    CK(cudaMallocAsync(&d, sizeof h, m->st));
+    CK(cudaMemcpyAsync(d, h, sizeof h, cudaMemcpyHostToDevice, m->st));
+    const exb_kv_view kv = kv_view_of(m);
+    const int rc = exb_kv_copy_pages(&kv, d, d + 1, d + 2, 1, nullptr, m->st);
+    CK(cudaFreeAsync(d, m->st));
+    if (rc) return rc;
+    CK(cudaStreamSynchronize(m->st));
+  }
+  m->seq_len[dst] = n;
+  return EXB_OK;
 }
 
 // The token buffer holds max_batch x max_seq tokens (no call can produce more), allocated once:

@@ -62,6 +62,7 @@ struct AttnArgs {
   const int64_t* qkv = nullptr; int ldqkv = 0;  // (R, (H + 2KV) hd) projected q|k|v (before RoPE)
   const int32_t* row_seq = nullptr;             // (R) sequence slot of each row
   const int32_t* row_pos = nullptr;             // (R) absolute position of each row
+  const int32_t* row_at = nullptr;              // rope_cache_rows: (R) cache position where it is not row_pos
   const int32_t* cos_t = nullptr;               // (Tmax, hd/2) Q16
   const int32_t* sin_t = nullptr;
   int16_t* kc = nullptr;                        // K cache (B, KV, Smax, hd) int16 (this layer)

@@ -331,7 +331,8 @@ EXB_DEV void rope_cache_rows(const AttnArgs& a, int first_task = 0, int stride =
   for (int t = first_task + warp; t < tasks; t += stride) {
     const int r = t / (a.KV + a.H), h = t - r * (a.KV + a.H);
     const int pos = a.row_pos[r], seq = a.row_seq[r];
-    if (pos < 0 || pos >= a.Smax || pos >= a.Tmax) {
+    const int at = a.row_at ? a.row_at[r] : pos;         // cache position (a tree's nodes: not the RoPE position)
+    if (pos < 0 || at < 0 || at >= a.Smax || pos >= a.Tmax) {
       if (lane == 0) set_err(a.err, ERR_BOUNDS);
       continue;
     }
@@ -355,7 +356,7 @@ EXB_DEV void rope_cache_rows(const AttnArgs& a, int first_task = 0, int stride =
     for (int o = 16; o > 0; o >>= 1) { const uint64_t w = __shfl_xor_sync(0xffffffffu, m, o); m = w > m ? w : m; }
     const int sh = qrow_shift(m);
     if (is_k) {
-      const size_t cidx = ((size_t)seq * a.KV + h) * a.Smax + pos;
+      const size_t cidx = ((size_t)seq * a.KV + h) * a.Smax + at;
       const int64_t* vrow = a.qkv + (size_t)r * a.ldqkv + (size_t)(a.H + a.KV + h) * hd;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {

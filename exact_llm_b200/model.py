@@ -17,7 +17,7 @@ import hashlib
 
 import numpy as np
 
-from . import tables
+from . import drafting, tables
 from ._lib import Config, check, lib, ptr
 
 LIN_NAMES = ("q", "k", "v", "o", "gate", "up", "down")
@@ -373,6 +373,69 @@ class ExactModel:
         for r in lg:
             chain = self._step_hash(chain, r)
         return (True, None) if chain == receipt["chain"] else (False, "chain")
+
+    # ------------------------------------------------------------------ drafted trees
+    def fork(self, src, dst, n=None):
+        """Copy the first ``n`` positions (all of them by default) of slot ``src`` to slot ``dst``: a prompt
+        shared by several continuations.  Returns the new Cache."""
+        n = lib.exb_seq_len(self.h, int(src)) if n is None else int(n)
+        check(lib.exb_seq_fork(self.h, int(src), int(dst), n))
+        return Cache(self, int(dst))
+
+    def tree_step(self, trees, u20=None, tnum=1 << 16, max_len=None, want_logits=False):
+        """One step of several sequences on trees of drafted tokens (exb_tree_step).  ``trees`` is a list of
+        (slot or Cache, ids, parents): node 0 is the sequence's next input token (parent -1), every other
+        node names an earlier one as its parent.  ``u20`` holds one random number per node, trees one after
+        another (None: greedy).  Returns per tree (accepted nodes, the target's token at each; the last one
+        is new), and with ``want_logits`` also the logits of all nodes, int64 (R, V)."""
+        slots = [t[0].slot if isinstance(t[0], Cache) else int(t[0]) for t in trees]
+        flat = [np.asarray([x for t in trees for x in t[k]], np.int32) for k in (1, 2)]
+        if len(flat[0]) != len(flat[1]) or any(len(t[1]) != len(t[2]) for t in trees):
+            raise ValueError("tree_step: as many parents as ids")
+        start = np.concatenate([[0], np.cumsum([len(t[1]) for t in trees])]).astype(np.int32)
+        B, R = len(trees), int(start[-1])
+        ml = int(max_len or max((len(t[1]) for t in trees), default=1))
+        u = None if u20 is None else np.ascontiguousarray(np.asarray(u20, np.int32).reshape(-1))
+        if u is not None and len(u) != R:
+            raise ValueError("tree_step: one random number per node")
+        seqs = np.asarray(slots, np.int32)
+        n, path, toks = np.empty(B, np.int32), np.empty((B, ml), np.int32), np.empty((B, ml), np.int32)
+        logits = np.empty((R, self.c["V"]), np.int64) if want_logits else None
+        self._rows = R
+        check(lib.exb_tree_step(self.h, B, ptr(seqs, ctypes.c_int32), ptr(start, ctypes.c_int32),
+                                ptr(flat[0], ctypes.c_int32), ptr(flat[1], ctypes.c_int32), ptr(u, ctypes.c_int32),
+                                int(tnum), ml, ptr(n, ctypes.c_int32), ptr(path, ctypes.c_int32),
+                                ptr(toks, ctypes.c_int32), None, ptr(logits, ctypes.c_int64)))
+        res = [(path[b, :n[b]].tolist(), toks[b, :n[b]].tolist()) for b in range(B)]
+        return (res, logits) if want_logits else res
+
+    def generate_drafted(self, prompt, n, draft=None, seed=None, temp=None, slot=0):
+        """``n`` tokens after ``prompt`` by steps on drafted trees: the tokens of greedy() (or, with ``seed``
+        and ``temp``, of generate_sampled()), in fewer steps the better the draft is.  ``draft(tokens)``
+        gets prompt and tokens so far and returns (ids, parents) of the nodes that may follow, parent -1 for
+        the ones after the last token; default ``drafting.ngram_tree``.  Returns (tokens, steps)."""
+        draft = draft or drafting.ngram_tree
+        tnum = 1 << 16 if temp is None else self.temp_num(temp)
+        cache = self.new_cache(slot)
+        lg = self.forward(prompt, cache, last_only=True)
+        prompt = [int(t) for t in prompt]
+        toks = [int(self.last_next[-1]) if seed is None else int(self.sample(lg, [seed], [0], tnum)[0])]
+        steps = 0
+        while len(toks) < n:
+            ids, par = draft(prompt + toks)
+            room = self.max_seq - cache.n
+            ids, par = [toks[-1]] + [int(t) for t in ids], [-1] + [int(p) + 1 for p in par]
+            ids, par = ids[:room], par[:room]
+            u = None
+            if seed is not None:
+                depth = []
+                for p in par:
+                    depth.append(0 if p < 0 else depth[p] + 1)
+                u = [drafting.u20(seed, len(toks) + d) for d in depth]
+            (_, new), = self.tree_step([(cache, ids, par)], u, tnum, max_len=min(len(ids), n - len(toks)))
+            toks += new
+            steps += 1
+        return toks, steps
 
     # ------------------------------------------------------------------ weightless cell verifier
     def verifier_keys(self, seed=2026):

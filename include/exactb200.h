@@ -195,6 +195,24 @@ int exb_generate(exb_model* m, int B, const int32_t* first_ids, int steps, int32
  * model's stream; no host synchronisation. */
 int exb_generate_device(exb_model* m, int B, const int32_t* ids_dev, int steps, int32_t* tokens_dev);
 
+/* One decoding step on drafted trees, without a counterpart in the reference (its GraphDecoder appends one
+ * token): every row of B different sequence slots runs through the model as one chunk (rows
+ * row_start[b] .. row_start[b+1]-1 are sequence seqs[b]'s tree, at most 512 rows in all, 256 for MoE;
+ * node 0 is the sequence's next input token, every other node's parent an earlier one, parent -1 for
+ * node 0), the target's token is chosen at every node (u20 as in exb_tree_verify, NULL: greedy), the
+ * agreeing path is accepted, its cache rows are moved together and the sequence grows by n[b].
+ * The tokens, logits and cache rows are those of one-token steps along the path, bit for bit.
+ * HOST buffers: n int32 (B), path and tokens int32 (B, max_len), sampled int32 (R) or NULL, logits
+ * int64 (R, V) or NULL.  Needs the tensor-core path (see "tc"): one GPU, V a multiple of 128, no trace,
+ * commitment or Freivalds capture. */
+int exb_tree_step(exb_model* m, int B, const int32_t* seqs, const int32_t* row_start, const int32_t* ids,
+                  const int32_t* parent, const int32_t* u20, int64_t tnum, int max_len, int32_t* n, int32_t* path,
+                  int32_t* tokens, int32_t* sampled, int64_t* logits);
+
+/* Copy the first n cached positions of slot src to slot dst in every layer; dst then holds n positions
+ * (a prompt shared by several continuations). */
+int exb_seq_fork(exb_model* m, int src, int dst, int n);
+
 /* KV cache export (exact_torch.py:140, 146-149: TModel's cache entries kq, sk, v; the static
  * GraphDecoder cache of experiments/speed_fair_kaggle.py:596-606, 617-618): positions 0..n-1 of
  * sequence slot `seq` at layer `layer`, into HOST buffers (any may be NULL):
