@@ -74,6 +74,36 @@ EXB_DEV void tmem_ld4(uint32_t taddr, int32_t* v) {
 EXB_DEV constexpr uint32_t tt_idesc(bool as, bool bs, int n) {
   return (2u << 4) | ((as ? 1u : 0u) << 7) | ((bs ? 1u : 0u) << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
+// stores to shared memory by 32-bit address
+EXB_DEV void sts64(uint32_t a, uint32_t x, uint32_t y) { asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(a), "r"(x), "r"(y) : "memory"); }
+EXB_DEV void sts32(uint32_t a, uint32_t x) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(x) : "memory"); }
+EXB_DEV void sts8(uint32_t a, uint32_t x) {
+  asm volatile("{\n .reg .b16 t;\n cvt.u16.u32 t, %1;\n st.shared.u8 [%0], t;\n}\n" ::"r"(a), "r"(x) : "memory");
+}
+// one MMA with its descriptors put together inside: low words base + constant, the common high word.  Few
+// registers live across a row of them (the MMA warp has 32; a spilled operand is a trip to L2)
+constexpr uint32_t TT_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);    // as tc_desc
+template <int DOFF, int AOFF, int BOFF, uint32_t IDESC>
+EXB_DEV void tt_mma(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b32 x, y, z, w;\n .reg .b64 da, db;\n"
+      " setp.ne.b32 p, %3, 0;\n add.u32 z, %0, %4;\n add.u32 x, %1, %5;\n add.u32 y, %2, %6;\n"
+      " mov.b32 w, %8;\n mov.b64 da, {x, w};\n mov.b64 db, {y, w};\n mov.b32 x, %7;\n"
+      " tcgen05.mma.cta_group::1.kind::i8 [z], da, db, x, p;\n}\n"
+      ::"r"(d), "r"(a), "r"(b), "r"((uint32_t)accumulate), "n"(DOFF), "n"(AOFF), "n"(BOFF), "n"(IDESC), "n"(TT_DESC_HI)
+      : "memory");
+}
+EXB_DEV uint32_t tt_desc_lo(const void* tile) { return ((smem_u32(tile) >> 4) & 0x3FFF) | (1u << 16); }
+// the K steps of one product
+template <int KS, int DOFF, int AOFF, int BOFF, uint32_t IDESC>
+EXB_DEV void tt_product(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
+  tt_mma<DOFF, AOFF, BOFF, IDESC>(d, a, b, accumulate);
+  if constexpr (KS > 1) tt_mma<DOFF, AOFF + 2, BOFF + 2, IDESC>(d, a, b, true);
+  if constexpr (KS > 2) {
+    tt_mma<DOFF, AOFF + 4, BOFF + 4, IDESC>(d, a, b, true);
+    tt_mma<DOFF, AOFF + 6, BOFF + 6, IDESC>(d, a, b, true);
+  }
+}
 EXB_DEV void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // 64-bit values in an order that an unsigned maximum keeps; 0 is below all of them
@@ -169,6 +199,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
   __shared__ uint64_t bar_s[2], bar_f[2], bar_k[2], bar_p;
   __shared__ uint32_t tmem_sh;
   __shared__ int qmax_sh;
+  __shared__ volatile int top_sh[2];                         // some p of the unit has a third digit
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const exb_kv_view& kv = a.kv;
 
@@ -179,6 +210,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
       mbar_init(&bar_k[i], TT_CW);
     }
     mbar_init(&bar_p, 1);
+    top_sh[0] = top_sh[1] = 0;
     mbar_fence_init();
   }
   if (warp == TT_CW) {
@@ -194,7 +226,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_sh;
+  const uint32_t tmem = tmem_sh, sb = smem_u32(sm);
   const int64_t* pre = w.pre + (PASS == 2 ? a.B + 1 : 0);
   const int64_t total = pre[a.B];
   int64_t u = total * blockIdx.x / gridDim.x;
@@ -213,20 +245,24 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
     asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     // ---- the MMA warp: one lane
     if (warp == TT_CW && lane == 0) {
+      const uint32_t qlo = tt_desc_lo(sm), klo = tt_desc_lo(sm + G::OFF_K), vlo = tt_desc_lo(sm + G::OFF_V),
+                     plo = tt_desc_lo(sm + G::OFF_P);
+      constexpr int QP = G::QB >> 4, KP = G::KB >> 4, VP = 16384 >> 4;       // planes, in 16 bytes
       auto issue_scores = [&](int sub, int kbuf, int col) {
-        const unsigned char* kd = sm + G::OFF_K + kbuf * 2 * G::KB;
-        const unsigned char* qd = sm + sub * 2 * G::QB;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) tc_mma_i8(tmem + col, tc_desc(kd, k), tc_desc(qd, k), tt_idesc(false, false, NT), k > 0);
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-          tc_mma_i8(tmem + col + NT, tc_desc(kd, k), tc_desc(qd + G::QB, k), tt_idesc(false, true, NT), k > 0);
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-          tc_mma_i8(tmem + col + NT, tc_desc(kd + G::KB, k), tc_desc(qd, k), tt_idesc(true, false, NT), true);
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-          tc_mma_i8(tmem + col + 2 * NT, tc_desc(kd + G::KB, k), tc_desc(qd + G::QB, k), tt_idesc(true, true, NT), k > 0);
+        const uint32_t k = klo + kbuf * 2 * KP, q = qlo + sub * 2 * QP, d = tmem + col;
+        tt_product<KS, 0, 0, 0, tt_idesc(false, false, NT)>(d, k, q, false);
+        tt_product<KS, NT, 0, QP, tt_idesc(false, true, NT)>(d, k, q, false);
+        tt_product<KS, NT, KP, 0, tt_idesc(true, false, NT)>(d, k, q, true);
+        tt_product<KS, 2 * NT, KP, QP, tt_idesc(true, true, NT)>(d, k, q, false);
+      };
+      // digit PD of p with the four of V; the first unit's first product of a weight starts it
+      auto products = [&](auto pd_t, bool more) {
+        constexpr int PD = decltype(pd_t)::value, D = G::ACC + PD * NT;
+        const uint32_t p = plo + PD * QP;
+        tt_product<4, D, 0, 0, tt_idesc(false, false, NT)>(tmem, vlo, p, more || PD > 0);
+        tt_product<4, D + NT, VP, 0, tt_idesc(false, false, NT)>(tmem, vlo, p, more || PD > 0);
+        tt_product<4, D + 2 * NT, 2 * VP, 0, tt_idesc(false, false, NT)>(tmem, vlo, p, more || PD > 0);
+        tt_product<4, D + 3 * NT, 3 * VP, 0, tt_idesc(true, false, NT)>(tmem, vlo, p, more);
       };
       while (u < uend) {
         const TtRun run = tt_run(a, pre, G::NR, u, uend);
@@ -259,15 +295,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
             }
             wait(bar_k, ph_k, 1);
             tc_fence_after();
-#pragma unroll 1
-            for (int pd = 0; pd < 3; ++pd)
-#pragma unroll
-              for (int vd = 0; vd < 4; ++vd)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  tc_mma_i8(tmem + G::ACC + (pd + vd) * NT, tc_desc(sm + G::OFF_V + vd * 16384, k),
-                            tc_desc(sm + G::OFF_P + pd * G::QB, k), tt_idesc(vd == 3, false, NT),
-                            i > 0 || k > 0 || !(pd == 0 || vd == 3));       // a weight's first product starts it
+            const bool top = top_sh[i & 1] || i == 0;        // (the first unit's products start every weight)
+            top_sh[i & 1] = 0;
+            products(std::integral_constant<int, 0>{}, i > 0);
+            products(std::integral_constant<int, 1>{}, i > 0);
+            if (top) products(std::integral_constant<int, 2>{}, i > 0);
             tc_commit(&bar_p);
           }
         }
@@ -362,19 +394,19 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
       };
       const int ko = kr * 128 + (((kc >> 1) ^ (kr & 7)) << 4) + (kc & 1) * 8;
       auto store_k = [&](int buf) {
-        unsigned char* d = sm + G::OFF_K + buf * 2 * G::KB + ko;
+        const uint32_t d = sb + G::OFF_K + buf * 2 * G::KB + ko;
 #pragma unroll
         for (int c = 0; c < KC; ++c)
           if (KALL || kr < TT_BK) {
             uint2 lo, hi;
             int16_digits(kraw[c], lo, hi);
-            *reinterpret_cast<uint2*>(d + c * KSTEP * 128) = lo;
-            *reinterpret_cast<uint2*>(d + G::KB + c * KSTEP * 128) = hi;
+            sts64(d + c * KSTEP * 128, lo.x, lo.y);
+            sts64(d + G::KB + c * KSTEP * 128, hi.x, hi.y);
           }
       };
       // V block n of this warp: 16 positions kg, 32 dims; lane: 4 dims (piece vc), positions 4 aq ..
       const int cl = lane & 7, aq = lane >> 3, kg = warp & 7, vc = (warp >> 3) * 8 + cl;
-      const int vo = vc * 128 + ((kg ^ (vc & 7)) << 4) + aq * 4;
+      const uint32_t va = sb + G::OFF_V + vc * 128 + ((kg ^ (vc & 7)) << 4) + aq * 4;
       auto load_v = [&](int i) {
         const TtPlace* p = ring + (i & (TT_RING - 1)) * TT_BK + kg * 16 + aq * 4;
 #pragma unroll
@@ -389,15 +421,16 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
 #pragma unroll
         for (int n = 0; n < VB; ++n) {
           if (HD >= 64 || vc < HD / 4) {
-            const uint32_t* x4 = reinterpret_cast<const uint32_t*>(&vraw[4 * n]);
+            const int4 x0 = vraw[4 * n], x1 = vraw[4 * n + 1], x2 = vraw[4 * n + 2], x3 = vraw[4 * n + 3];
+            uint32_t o4[4][4];
+            byte_planes(x0.x, x1.x, x2.x, x3.x, o4[0]);
+            byte_planes(x0.y, x1.y, x2.y, x3.y, o4[1]);
+            byte_planes(x0.z, x1.z, x2.z, x3.z, o4[2]);
+            byte_planes(x0.w, x1.w, x2.w, x3.w, o4[3]);
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-              uint32_t o4[4];
-              byte_planes(x4[d], x4[4 + d], x4[8 + d], x4[12 + d], o4);
+            for (int d = 0; d < 4; ++d)
 #pragma unroll
-              for (int p = 0; p < 4; ++p)
-                *reinterpret_cast<uint32_t*>(sm + G::OFF_V + p * 16384 + (d * RS + 16 * n) * 128 + vo) = o4[p];
-            }
+              for (int p = 0; p < 4; ++p) sts32(va + p * 16384 + (d * RS + 16 * n) * 128, o4[d][p]);
           }
         }
       };
@@ -599,8 +632,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
         const int qmax = qmax_sh;
         const int live = max(0, min(RPT, ng - cg * RPT));    // this thread's rows that exist
         // row r of column group cg is row 4 r + cg of the P planes: two places of the key in them
-        const int p0 = cg * 128 + (((key >> 4) ^ cg) << 4) + (key & 15);
-        const int p1 = cg * 128 + (((key >> 4) ^ (4 + cg)) << 4) + (key & 15);
+        const uint32_t p0 = sb + G::OFF_P + cg * 128 + (((key >> 4) ^ cg) << 4) + (key & 15);
+        const uint32_t p1 = sb + G::OFF_P + cg * 128 + (((key >> 4) ^ (4 + cg)) << 4) + (key & 15);
 #pragma unroll 1
         for (int i = 0; i < nk; ++i) {
           const int t = (kt0 + i) * TT_BK + key;
@@ -639,15 +672,18 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
           tc_fence_before();
           arrive(&bar_f[0]);                                 // the next unit's scores may come
           if (i > 0) wait(&bar_p, ph_p, 0);                  // V, P and the other key buffer are free
+          uint32_t big = 0;
 #pragma unroll
           for (int r = 0; r < RPT; ++r) {
             if (r < live) {
-              unsigned char* d = sm + G::OFF_P + r * 512 + ((r & 1) ? p1 : p0);
-              d[0] = (unsigned char)pr[r];
-              d[G::QB] = (unsigned char)(pr[r] >> 8);
-              d[2 * G::QB] = (unsigned char)(pr[r] >> 16);
+              const uint32_t d = ((r & 1) ? p1 : p0) + r * 512;
+              sts8(d, pr[r]);
+              sts8(d + G::QB, pr[r] >> 8);
+              sts8(d + 2 * G::QB, pr[r] >> 16);
+              big |= pr[r];
             }
           }
+          if (__any_sync(0xffffffffu, big >> 16) && lane == 0) top_sh[i & 1] = 1;
           store_v();
           if (i + 2 < nk) store_k(i & 1);
           put_place(i + TT_AHEAD);
