@@ -11,9 +11,10 @@
 //               the whole run of units (at most 3 * 255^2 * 8064 positions < 2^31)
 //   digits      cache rows come through registers: K in 16-byte pieces, V in blocks of 4 positions x 4
 //               dims that byte permutations turn into words of 4 positions per digit
-//   warps       16 compute warps (TMEM lane = position, four column groups) and one that issues the MMAs;
-//               they meet on mbarriers only, so the loads, the digits, the MMAs and the softmax of
-//               neighbouring units overlap
+//   warps       16 compute warps (TMEM lane = position, four column groups), three that issue the MMAs (one
+//               alone took 90 cycles an MMA next to the compute warps, twice what the tensor core takes) and
+//               one that looks up the pages; they meet on mbarriers only, so the look-ups, the loads, the
+//               digits, the MMAs and the softmax of neighbouring units overlap
 // Scores are computed anew in each kernel: keeping them would move 12 bytes a score, more than the MMAs
 // and the three multiply-adds that make one cost.
 #include <algorithm>
@@ -28,13 +29,17 @@ namespace exb {
 
 constexpr int TT_CW = 16;                          // compute warps
 constexpr int TT_COMPUTE = 32 * TT_CW;
-constexpr int TT_THREADS = TT_COMPUTE + 128;       // and a group of warps whose first issues the MMAs
+constexpr int TT_THREADS = TT_COMPUTE + 128;       // and four: MMAs (two or three), places
 constexpr int TT_BK = 128;                         // positions per unit
 constexpr int TT_CHUNK = 32;                       // a chunk is 32 to 63 units of positions (all, if fewer): its row
                                                    // tiles follow one another, so its cache rows are read from L2
                                                    // by all but the first; a run is a part of a chunk
 constexpr int TT_RING = 8;                         // units whose rows' places are kept
-constexpr int TT_AHEAD = 5;                        // a unit's places are written this many units earlier
+
+struct TtPlaces {                                  // where a unit's cache rows lie, in elements, and the shifts
+  int64_t k[TT_BK], v[TT_BK];
+  int s[TT_BK];                                    // -1: there is no such position (the places are some row's)
+};
 
 template <int PASS>
 struct TtGeo {
@@ -49,12 +54,8 @@ struct TtGeo {
   static constexpr int OFF_P = OFF_V + (PASS == 2 ? 4 * 16384 : 0);
   static constexpr int OFF_T = OFF_P + (PASS == 2 ? 3 * QB : 0);
   static constexpr int OFF_RING = OFF_T + (PASS ? 41088 : 0);
-  static constexpr int SMEM = OFF_RING + TT_RING * TT_BK * 24 + 1024;
+  static constexpr int SMEM = OFF_RING + TT_RING * (int)sizeof(TtPlaces) + 1024;
   static constexpr int ACC = 3 * NT;               // first column of the p . v accumulators
-};
-
-struct TtPlace {                                   // a position's rows in the cache, in elements
-  int64_t k, v, s;                                 // s = -1: there is no such position
 };
 
 struct TtRow {
@@ -189,17 +190,20 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   int32_t* T = reinterpret_cast<int32_t*>(sm + G::OFF_T);
-  TtPlace* ring = reinterpret_cast<TtPlace*>(sm + G::OFF_RING);
+  TtPlaces* ring = reinterpret_cast<TtPlaces*>(sm + G::OFF_RING);
   __shared__ TtRow rowc[G::NR];
   __shared__ const uint64_t* rmask[G::NR];
   __shared__ int64_t rmax[PASS ? G::NR : 1];
   __shared__ int64_t rowq[G::NR];                            // row of q, qs and out
-  // bar_s: a score tile is complete; bar_f: every warp has read it; bar_k: a unit's keys (PASS 2: and its P
-  // and V) are in place; bar_p: the p . v products of a unit are complete
-  __shared__ uint64_t bar_s[2], bar_f[2], bar_k[2], bar_p;
+  // bar_s: a score tile is complete; bar_f: every warp has read it; bar_k: a unit's keys are in place (PASS 2:
+  // its P and V and the keys of the next but one); bar_q: a run's first keys (PASS 2); bar_p: the p . v
+  // products of a unit are complete.  A waiter never falls two phases behind: what comes two phases later
+  // depends on what it does after its wait.
+  // ring_full, ring_free: a unit's places are written, every warp is done with them
+  __shared__ uint64_t bar_s[2], bar_f[2], bar_k[2], bar_p, bar_q, ring_full[TT_RING], ring_free[TT_RING];
   __shared__ uint32_t tmem_sh;
   __shared__ int qmax_sh;
-  __shared__ volatile int top_sh[2];                         // some p of the unit has a third digit
+  __shared__ volatile uint32_t top_sh[2];                    // the last unit (+ 1) with a third digit in some p
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const exb_kv_view& kv = a.kv;
 
@@ -209,7 +213,12 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
       mbar_init(&bar_f[i], TT_CW);
       mbar_init(&bar_k[i], TT_CW);
     }
-    mbar_init(&bar_p, 1);
+    for (int i = 0; i < TT_RING; ++i) {
+      mbar_init(&ring_full[i], 1);
+      mbar_init(&ring_free[i], TT_CW);
+    }
+    mbar_init(&bar_q, TT_CW);
+    mbar_init(&bar_p, 2);                                    // two warps issue the products
     top_sh[0] = top_sh[1] = 0;
     mbar_fence_init();
   }
@@ -233,18 +242,74 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
   const int64_t uend = total * (blockIdx.x + 1) / gridDim.x;
   bool late = false;                                         // a wait gave up
   // parity of the next completion of each barrier, as this thread waits for them
-  uint32_t ph_s = 0, ph_f = 0, ph_k = 0, ph_p = 0;           // bit i: barrier i
+  uint32_t ph_s = 0, ph_f = 0, ph_q = 0, ph_p = 0;           // bit i: barrier i
   auto wait = [&](uint64_t* bar, uint32_t& ph, int i) {
     late |= !mbar_wait(bar + i, (ph >> i) & 1, TC_WAIT_LIMIT);
     ph ^= 1u << i;
   };
   uint32_t tiles = 0, units = 0;                             // of this CTA so far
+  auto wait_k = [&](uint32_t unit) { late |= !mbar_wait(&bar_k[unit & 1], (unit >> 1) & 1, TC_WAIT_LIMIT); };
 
-  // 640 threads start with 96 registers each, 61440 in all; 128 x 32 + 512 x 112 = 61440
+  // 640 threads start with 96 registers each, 61440 in all; 128 x 48 + 512 x 104 = 59392
   if (warp >= TT_CW) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
-    // ---- the MMA warp: one lane
-    if (warp == TT_CW && lane == 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    const int role = warp - TT_CW;
+    if (role == 3) {
+      // ---- places: four positions a lane; the pages of the next unit are looked up meanwhile
+      const int32_t* trow = nullptr;
+      int pg[4], S = 0, j = 0, t0 = 0;
+      TtRun run;
+      int i = 0;                                             // unit of the run whose pages are in pg
+      auto next_pages = [&]() {                              // false: there are no more units
+        if (i >= run.nk) {
+          if (u >= uend) return false;
+          run = tt_run(a, pre, G::NR, u, uend);
+          u += run.nk;
+          i = 0;
+          S = tree_seq(a, run.b, false).S;
+          trow = a.table + (size_t)run.b * a.MP;
+        }
+        j = run.j;
+        t0 = (run.kt0 + i) * TT_BK + lane;
+        ++i;
+#pragma unroll
+        for (int f = 0; f < 4; ++f) pg[f] = t0 + 32 * f < S ? __ldg(trow + div_by(t0 + 32 * f, a.page_div)) : -1;
+        return true;
+      };
+      bool more = next_pages();
+      while (more) {
+        const uint32_t slot = units % TT_RING;
+        TtPlaces& out = ring[slot];
+        int64_t k[4], v[4];
+        int sh[4];
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          const int t = t0 + 32 * f, off = t - div_by(t, a.page_div) * kv.page;
+          k[f] = v[f] = 0;
+          sh[f] = -1;
+          if ((unsigned)pg[f] < (unsigned)kv.pages) {
+            k[f] = pg[f] * kv.k_page + off * kv.k_pos + j * kv.k_head;
+            v[f] = pg[f] * kv.v_page + off * kv.v_pos + j * kv.v_head;
+            sh[f] = (uint8_t)__ldg(kv.ks + pg[f] * kv.s_page + off * kv.s_pos + j * kv.s_head);
+          } else if (t < S) {
+            set_err(a.status, ERR_BOUNDS);
+          }
+        }
+        more = next_pages();
+        if (units >= TT_RING) late |= !mbar_wait(&ring_free[slot], ((units / TT_RING) & 1) ^ 1, TC_WAIT_LIMIT);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          out.k[lane + 32 * f] = k[f];
+          out.v[lane + 32 * f] = v[f];
+          out.s[lane + 32 * f] = sh[f];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ring_full[slot]);
+        ++units;
+      }
+    } else if (lane == 0) {
+      // ---- MMAs, one lane.  Scores: warp 16, with two score tiles warps 16 and 17, a TMEM buffer each;
+      // p . v: warps 17 and 18, half of the weights each
       const uint32_t qlo = tt_desc_lo(sm), klo = tt_desc_lo(sm + G::OFF_K), vlo = tt_desc_lo(sm + G::OFF_V),
                      plo = tt_desc_lo(sm + G::OFF_P);
       constexpr int QP = G::QB >> 4, KP = G::KB >> 4, VP = 16384 >> 4;       // planes, in 16 bytes
@@ -255,15 +320,15 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
         tt_product<KS, NT, KP, 0, tt_idesc(true, false, NT)>(d, k, q, true);
         tt_product<KS, 2 * NT, KP, QP, tt_idesc(true, true, NT)>(d, k, q, false);
       };
-      // digit PD of p with the four of V; the first unit's first product of a weight starts it
-      auto products = [&](auto pd_t, bool more) {
-        constexpr int PD = decltype(pd_t)::value, D = G::ACC + PD * NT;
-        const uint32_t p = plo + PD * QP;
-        tt_product<4, D, 0, 0, tt_idesc(false, false, NT)>(tmem, vlo, p, more || PD > 0);
-        tt_product<4, D + NT, VP, 0, tt_idesc(false, false, NT)>(tmem, vlo, p, more || PD > 0);
-        tt_product<4, D + 2 * NT, 2 * VP, 0, tt_idesc(false, false, NT)>(tmem, vlo, p, more || PD > 0);
-        tt_product<4, D + 3 * NT, 3 * VP, 0, tt_idesc(true, false, NT)>(tmem, vlo, p, more);
+      // digit PD of p times digit VD of V, added to weight PD + VD
+      auto product = [&](auto pd_t, auto vd_t, bool add) {
+        constexpr int PD = decltype(pd_t)::value, VD = decltype(vd_t)::value;
+        tt_product<4, G::ACC + (PD + VD) * NT, VD * VP, PD * QP, tt_idesc(VD == 3, false, NT)>(tmem, vlo, plo, add);
       };
+      using C0 = std::integral_constant<int, 0>;
+      using C1 = std::integral_constant<int, 1>;
+      using C2 = std::integral_constant<int, 2>;
+      using C3 = std::integral_constant<int, 3>;
       while (u < uend) {
         const TtRun run = tt_run(a, pre, G::NR, u, uend);
         u += run.nk;
@@ -271,35 +336,55 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
           const TreeSeq sq = tree_seq(a, run.b, false);
           const int nh = sq.T * a.rep - run.rt * G::NR > NT ? 2 : 1;
           for (int i = 0; i < run.nk; ++i, ++units) {
-            wait(bar_k, ph_k, units & 1);
             for (int h = 0; h < nh; ++h, ++tiles) {
               const int s = tiles & 1;
+              if (role != s) continue;
+              wait_k(units);
               if (tiles >= 2) wait(bar_f, ph_f, s);
               tc_fence_after();
               issue_scores(h, units & 1, s * 3 * NT);
               tc_commit(&bar_s[s]);
             }
           }
-        } else {
-          // bar_k[0]: the run's first keys; bar_k[1]: P and V of a unit, and the keys of the next but one
-          wait(bar_k, ph_k, 0);
+        } else if (role == 0) {
+          wait(&bar_q, ph_q, 0);
           tc_fence_after();
           issue_scores(0, 0, 0);
           tc_commit(&bar_s[0]);
-          for (int i = 0; i < run.nk; ++i) {
+          for (int i = 0; i < run.nk; ++i, ++units) {
+            if (i > 0 && i + 1 < run.nk) wait_k(units - 1);  // the keys of unit i + 1
             wait(bar_f, ph_f, 0);
             if (i + 1 < run.nk) {
               tc_fence_after();
               issue_scores(0, (i + 1) & 1, 0);
               tc_commit(&bar_s[0]);
             }
-            wait(bar_k, ph_k, 1);
+          }
+        } else {
+          for (int i = 0; i < run.nk; ++i, ++units) {
+            wait_k(units);
             tc_fence_after();
-            const bool top = top_sh[i & 1] || i == 0;        // (the first unit's products start every weight)
-            top_sh[i & 1] = 0;
-            products(std::integral_constant<int, 0>{}, i > 0);
-            products(std::integral_constant<int, 1>{}, i > 0);
-            if (top) products(std::integral_constant<int, 2>{}, i > 0);
+            const bool add = i > 0;                          // the first unit's first product of a weight starts it
+            const bool top = !add || top_sh[units & 1] == units + 1;
+            if (role == 1) {
+              product(C0{}, C0{}, add);
+              product(C0{}, C3{}, add);
+              product(C1{}, C2{}, true);
+              product(C1{}, C3{}, add);
+              if (top) {
+                product(C2{}, C1{}, true);
+                product(C2{}, C2{}, true);
+              }
+            } else {
+              product(C0{}, C1{}, add);
+              product(C1{}, C0{}, true);
+              product(C0{}, C2{}, add);
+              product(C1{}, C1{}, true);
+              if (top) {
+                product(C2{}, C0{}, true);
+                product(C2{}, C3{}, add);
+              }
+            }
             tc_commit(&bar_p);
           }
         }
@@ -307,7 +392,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
     }
     __syncwarp();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     const int quarter = warp & 3, cg = warp >> 2;            // TMEM lanes 32 quarter .., rows RPT cg ..
     const int key = quarter * 32 + lane;
     const uint32_t tlane = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -323,27 +408,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
       u += nk;
       const int g0 = run.rt * G::NR, ng = min(G::NR, sq.T * a.rep - g0);
       const int nh = PASS < 2 && ng > NT ? 2 : 1;
-      const int32_t* trow = a.table + (size_t)run.b * a.MP;
-      const int64_t kh = run.j * kv.k_head, vh = run.j * kv.v_head, sh0 = run.j * kv.s_head;
-      auto place = [&](int pg, int off) {                    // where an offset of a page lies
-        TtPlace p = {0, 0, -1};                              // (a position that is not there: some row, hidden)
-        if (pg >= 0) {
-          p.k = pg * kv.k_page + off * kv.k_pos + kh;
-          p.v = pg * kv.v_page + off * kv.v_pos + vh;
-          p.s = pg * kv.s_page + off * kv.s_pos + sh0;
-        }
-        return p;
-      };
       named_sync(1, TT_COMPUTE);                             // the last run is done with shared memory
       if (tid == 0) qmax_sh = 0;
-      for (int e = tid; e < TT_AHEAD * TT_BK; e += TT_COMPUTE) {
-        const int t = kt0 * TT_BK + e;
-        if (e < nk * TT_BK) {
-          int off = 0;
-          const int pg = t < sq.S ? page_of(a, trow, t, off) : -1;
-          ring[e] = place(pg, off);
-        }
-      }
       if (tid < G::NR && tid < ng) {                         // row i of the tile: node (g0 + i) / rep
         const int node = (g0 + tid) / a.rep;
         rowq[tid] = (int64_t)(sq.r0 + node) * a.H + (int64_t)run.j * a.rep + (g0 + tid - node * a.rep);
@@ -386,11 +452,18 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
       int4 vraw[PASS == 2 ? VB * 4 : 1];
       const int kr = tid / KCH, kc = tid % KCH;              // first key and piece, then KSTEP keys on
       constexpr int KSTEP = TT_COMPUTE / KCH;
-      auto load_k = [&](int i) {
-        const TtPlace* p = ring + (i & (TT_RING - 1)) * TT_BK + kr;
+      const uint32_t g = units;                              // the run's first unit
+      auto places = [&](int i) -> const TtPlaces& { return ring[(g + i) % TT_RING]; };
+      auto await_places = [&](int i) {
+        late |= !mbar_wait(&ring_full[(g + i) % TT_RING], ((g + i) / TT_RING) & 1, TC_WAIT_LIMIT);
+        __syncwarp();
+      };
+      auto load_k = [&](int i) {                             // (waits for the unit's places)
+        await_places(i);
+        const int64_t* p = places(i).k + kr;
 #pragma unroll
         for (int c = 0; c < KC; ++c)
-          if (KALL || kr < TT_BK) kraw[c] = __ldg(reinterpret_cast<const int4*>(kv.k + p[c * KSTEP].k) + kc);
+          if (KALL || kr < TT_BK) kraw[c] = __ldg(reinterpret_cast<const int4*>(kv.k + p[c * KSTEP]) + kc);
       };
       const int ko = kr * 128 + (((kc >> 1) ^ (kr & 7)) << 4) + (kc & 1) * 8;
       auto store_k = [&](int buf) {
@@ -408,10 +481,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
       const int cl = lane & 7, aq = lane >> 3, kg = warp & 7, vc = (warp >> 3) * 8 + cl;
       const uint32_t va = sb + G::OFF_V + vc * 128 + ((kg ^ (vc & 7)) << 4) + aq * 4;
       auto load_v = [&](int i) {
-        const TtPlace* p = ring + (i & (TT_RING - 1)) * TT_BK + kg * 16 + aq * 4;
+        const int64_t* p = places(i).v + kg * 16 + aq * 4;
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
-          const int4* at = reinterpret_cast<const int4*>(kv.v + p[f].v) + vc;
+          const int4* at = reinterpret_cast<const int4*>(kv.v + p[f]) + vc;
 #pragma unroll
           for (int n = 0; n < VB; ++n)
             if (HD >= 64 || vc < HD / 4) vraw[4 * n + f] = __ldg(at + 16 * n);
@@ -434,30 +507,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
           }
         }
       };
-      // shift of this thread's key in unit i; -1: no such position
-      auto key_shift = [&](int i) {
-        const int64_t s = ring[(i & (TT_RING - 1)) * TT_BK + key].s;
-        return s < 0 ? -1 : (int)(uint8_t)__ldg(kv.ks + s);
-      };
-      // a unit's pages are looked up one unit before its places are written
-      int pg_next = -1;
-      auto look_up = [&](int i) {
-        const int t = (kt0 + i) * TT_BK + tid;
-        pg_next = -1;
-        if (tid < TT_BK && i < nk && t < sq.S) pg_next = __ldg(trow + div_by(t, a.page_div));
-      };
-      auto put_place = [&](int i) {
-        if (tid < TT_BK && i < nk) {
-          const int t = (kt0 + i) * TT_BK + tid;
-          TtPlace p = {0, 0, -1};
-          if (t < sq.S) {
-            if ((unsigned)pg_next < (unsigned)kv.pages) p = place(pg_next, t - div_by(t, a.page_div) * kv.page);
-            else set_err(a.status, ERR_BOUNDS);
-          }
-          ring[(i & (TT_RING - 1)) * TT_BK + tid] = p;
-        }
-      };
-
       // ---- a score's sums put together, sh = qs + ks: n = 32 - sh, so the 64-bit sum shifted left by sh has the
       // score in its high words.  MODE 0: every position visible and sh in [0, 13], |score| < 2^31; MODE 1: sh
       // in [0, 31], with the mask and 64-bit distances; MODE 2: any shift
@@ -511,12 +560,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
           arrive(&bar_k[(units + 1) & 1]);
         }
         if (nk > 2) load_k(2);
-        int ksh = key_shift(0), ksh_next = -1;
-        look_up(TT_AHEAD);
         const int qmax = qmax_sh;
 #pragma unroll 1
         for (int i = 0; i < nk; ++i, ++units) {
-          if (i + 1 < nk) ksh_next = key_shift(i + 1);
+          const int ksh = places(i).s[key];                  // shift of this thread's key; -1: no such position
           const int t = (kt0 + i) * TT_BK + key;
           const int mode = mode_of(ksh, t, qmax);
 #pragma unroll
@@ -593,13 +640,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
           }
           if (i + 2 < nk) {                                  // the unit's keys are read: the next but one in their place
             store_k(units & 1);
-            put_place(i + TT_AHEAD);
             fence_async_smem();
             arrive(&bar_k[units & 1]);
             if (i + 3 < nk) load_k(i + 3);
-            look_up(i + TT_AHEAD + 1);
           }
-          ksh = ksh_next;
+          arrive(&ring_free[units % TT_RING]);
         }
         // the run's maxima and sums, over the warp's keys
 #pragma unroll
@@ -624,18 +669,17 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
         if (nk > 1) { load_k(1); store_k(1); }
         fence_async_smem();
         named_sync(1, TT_COMPUTE);
-        arrive(&bar_k[0]);
+        arrive(&bar_q);
         load_v(0);
         if (nk > 2) load_k(2);
-        int ksh = key_shift(0);
-        look_up(TT_AHEAD);
         const int qmax = qmax_sh;
         const int live = max(0, min(RPT, ng - cg * RPT));    // this thread's rows that exist
         // row r of column group cg is row 4 r + cg of the P planes: two places of the key in them
         const uint32_t p0 = sb + G::OFF_P + cg * 128 + (((key >> 4) ^ cg) << 4) + (key & 15);
         const uint32_t p1 = sb + G::OFF_P + cg * 128 + (((key >> 4) ^ (4 + cg)) << 4) + (key & 15);
 #pragma unroll 1
-        for (int i = 0; i < nk; ++i) {
+        for (int i = 0; i < nk; ++i, ++units) {
+          const int ksh = places(i).s[key];                  // shift of this thread's key; -1: no such position
           const int t = (kt0 + i) * TT_BK + key;
           const int mode = mode_of(ksh, t, qmax);
           uint32_t pr[RPT];                                  // p of this key for the thread's rows
@@ -683,18 +727,14 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
               big |= pr[r];
             }
           }
-          if (__any_sync(0xffffffffu, big >> 16) && lane == 0) top_sh[i & 1] = 1;
+          if (__any_sync(0xffffffffu, big >> 16) && lane == 0) top_sh[units & 1] = units + 1;
           store_v();
           if (i + 2 < nk) store_k(i & 1);
-          put_place(i + TT_AHEAD);
           fence_async_smem();
-          arrive(&bar_k[1]);
-          if (i + 1 < nk) {
-            load_v(i + 1);
-            if (i + 3 < nk) load_k(i + 3);
-            ksh = key_shift(i + 1);
-            look_up(i + TT_AHEAD + 1);
-          }
+          arrive(&bar_k[units & 1]);
+          if (i + 1 < nk) load_v(i + 1);
+          if (i + 3 < nk) load_k(i + 3);
+          arrive(&ring_free[units % TT_RING]);
         }
         wait(&bar_p, ph_p, 0);
         __syncwarp();
