@@ -318,7 +318,9 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
         const uint64_t d = (uint64_t)m - (uint64_t)lmax[i];
         base[i] = d < (1ull << 30) ? (int)d : (1 << 30);
       } else {
-        base[i] = m > INT32_MAX ? INT32_MAX : (int)m;        // another CTA's row may be far above
+        // another CTA's scores may be far above; 32-bit ones are above -1.6e9, so a lower maximum has none
+        // here, and 0 keeps the hidden ones far
+        base[i] = m > INT32_MAX ? INT32_MAX : m < -(3ll << 29) ? 0 : (int)m;
       }
     }
   }

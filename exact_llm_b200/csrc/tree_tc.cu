@@ -71,6 +71,12 @@ EXB_DEV void tmem_ld4(uint32_t taddr, int32_t* v) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = (int32_t)r[i];
 }
+// the loads into these registers are complete (they pass through, so no use of them moves before)
+EXB_DEV void tmem_wait12(int (&a)[4], int (&b)[4], int (&c)[4]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(b[0]), "+r"(b[1]), "+r"(b[2]), "+r"(b[3]), "+r"(c[0]),
+                 "+r"(c[1]), "+r"(c[2]), "+r"(c[3])::"memory");
+}
 // int32 sums, A and B signed or not, both K-major, M = 128
 EXB_DEV constexpr uint32_t tt_idesc(bool as, bool bs, int n) {
   return (2u << 4) | ((as ? 1u : 0u) << 7) | ((bs ? 1u : 0u) << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
@@ -151,6 +157,11 @@ __global__ void __launch_bounds__(256) k_tt_finish(int64_t* out, int64_t n) {
 struct TtRun {
   int b = 0, j = 0, rt = 0, kt0 = 0, nk = 0;
 };
+// units of positions in a chunk: near equal parts of 32 to 63
+EXB_DEV int tt_chunk(int nkt) {
+  const int n = max(1, nkt / TT_CHUNK);
+  return (nkt + n - 1) / n;
+}
 EXB_DEV TtRun tt_run(const TreeArgs& a, const int64_t* pre, int NR, int64_t u, int64_t uend) {
   TtRun r;
   int lo = 0, hi = a.B - 1;                                  // last sequence that begins at or before u
@@ -163,16 +174,15 @@ EXB_DEV TtRun tt_run(const TreeArgs& a, const int64_t* pre, int NR, int64_t u, i
   const TreeSeq sq = tree_seq(a, lo, false);
   const int nrt = (sq.T * a.rep + NR - 1) / NR, nkt = (sq.S + TT_BK - 1) / TT_BK;
   const int64_t x = u - pre[lo], per_head = (int64_t)nrt * nkt;
-  r.j = (int)(x / per_head);
+  // (a 64-bit division takes longer than the rest of this)
+  r.j = (int)(x < (1ll << 31) && per_head < (1ll << 31) ? (int)x / (int)per_head : x / per_head);
   const int64_t y = x - r.j * per_head;
-  const int nch = max(1, nkt / TT_CHUNK);
-  auto first = [&](int c) { return (int)((int64_t)nkt * c / nch); };       // first unit of positions of chunk c
-  int ch = (int)min((int64_t)(nch - 1), y / nrt * nch / nkt);
-  while (ch + 1 < nch && (int64_t)first(ch + 1) * nrt <= y) ++ch;
-  while ((int64_t)first(ch) * nrt > y) --ch;
-  const int len = first(ch + 1) - first(ch), z = (int)(y - (int64_t)first(ch) * nrt), k0 = z % len;
+  const int L = tt_chunk(nkt);
+  const int64_t chunk = (int64_t)L * nrt;
+  const int ch = (int)(y < (1ll << 31) ? (int)min(chunk, (int64_t)INT32_MAX) > (int)y ? 0 : (int)y / (int)chunk : y / chunk);
+  const int len = min(L, nkt - ch * L), z = (int)(y - ch * chunk), k0 = z % len;
   r.rt = z / len;
-  r.kt0 = first(ch) + k0;
+  r.kt0 = ch * L + k0;
   r.nk = (int)min((int64_t)(len - k0), uend - u);
   return r;
 }
@@ -195,6 +205,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
   __shared__ const uint64_t* rmask[G::NR];
   __shared__ int64_t rmax[PASS ? G::NR : 1];
   __shared__ int64_t rowq[G::NR];                            // row of q, qs and out
+  __shared__ unsigned long long row_sh[PASS < 2 ? G::NR : 1];
   // bar_s: a score tile is complete; bar_f: every warp has read it; bar_k: a unit's keys are in place (PASS 2:
   // its P and V and the keys of the next but one); bar_q: a run's first keys (PASS 2); bar_p: the p . v
   // products of a unit are complete.  A waiter never falls two phases behind: what comes two phases later
@@ -434,7 +445,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
           r.qs = a.qs[qi];
           if (PASS) {
             const int64_t m = tt_value(w.rowmax[qi]);
-            r.base = m > INT32_MAX ? INT32_MAX : (int)m;
+            // (32-bit scores are above -1.6e9: a lower maximum has none, and 0 keeps hidden ones far)
+            r.base = m > INT32_MAX ? INT32_MAX : m < -(3ll << 29) ? 0 : (int)m;
             rmax[tid] = m;
           }
           if (PASS == 2) {
@@ -508,8 +520,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
         }
       };
       // ---- a score's sums put together, sh = qs + ks: n = 32 - sh, so the 64-bit sum shifted left by sh has the
-      // score in its high words.  MODE 0: every position visible and sh in [0, 13], |score| < 2^31; MODE 1: sh
-      // in [0, 31], with the mask and 64-bit distances; MODE 2: any shift
+      // score in its high words.  MODE 0: every position visible and sh in [0, 13], |score| < 2^31; MODE 3: the
+      // same with the mask (a hidden score is INT32_MIN, 2^29 or more from any base); MODE 1: sh in [0, 31], with
+      // the mask and 64-bit distances; MODE 2: any shift
       auto sum64 = [&](int ll, int md, int hh, int sh) {     // sh in [0, 31]: with the rounding half
         return mad_wide_s32(hh, c2, mad_wide_s32(md, c1, mad_wide_s32(ll, c0, (int64_t)(0x80000000u >> sh))));
       };
@@ -525,7 +538,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
         return shr64((int64_t)((uint64_t)acc * (uint64_t)a.inv), 32 - sh);
       };
       auto mode_of = [&](int ksh, int t, int qmax) {
-        if (__all_sync(0xffffffffu, ksh >= 0 && ksh + qmax <= 13 && t < sq.ctx)) return 0;
+        if (__all_sync(0xffffffffu, ksh + qmax <= 13)) return __all_sync(0xffffffffu, ksh >= 0 && t < sq.ctx) ? 0 : 3;
         return __all_sync(0xffffffffu, ksh + qmax <= 31) ? 1 : 2;
       };
       auto seen = [&](int i, int ksh, int t) {               // row i of the unit, this thread's key
@@ -582,13 +595,24 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
                   tmem_ld4(col + r0, ll);
                   tmem_ld4(col + NT + r0, md);
                   tmem_ld4(col + 2 * NT + r0, hh);
-                  tmem_wait_ld();
+                  tmem_wait12(ll, md, hh);
                   int way = mode;
                   if (way == 0) {
 #pragma unroll
                     for (int f = 0; f < 4; ++f) {
                       const TtRow rc = rowc[h * NT + cg * RPT + r0 + f];
                       const int sh = rc.qs + ksh, sc = high(sum64(ll[f], md[f], hh[f], sh), sh);
+                      if (PASS == 0) mx[h][r0 + f] = max(mx[h][r0 + f], sc);
+                      else es[h][r0 + f] += exp_sm_flat(T, (uint32_t)rc.base - (uint32_t)sc);
+                    }
+                  }
+                  if (way == 3) {
+#pragma unroll
+                    for (int f = 0; f < 4; ++f) {
+                      const int i2 = h * NT + cg * RPT + r0 + f;
+                      const TtRow rc = rowc[i2];
+                      const int sh = rc.qs + max(ksh, 0);
+                      const int sc = seen(i2, ksh, t) ? high(sum64(ll[f], md[f], hh[f], sh), sh) : INT32_MIN;
                       if (PASS == 0) mx[h][r0 + f] = max(mx[h][r0 + f], sc);
                       else es[h][r0 + f] += exp_sm_flat(T, (uint32_t)rc.base - (uint32_t)sc);
                     }
@@ -646,23 +670,37 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
           }
           arrive(&ring_free[units % TT_RING]);
         }
-        // the run's maxima and sums, over the warp's keys
+        // the run's maxima and sums: over the warp's keys, lane r of a warp keeping row r's, over the four warps
+        // of a column group in shared memory, then one atomic a row
+        for (int i = tid; i < G::NR; i += TT_COMPUTE) row_sh[i] = 0;
+        named_sync(1, TT_COMPUTE);
 #pragma unroll
-        for (int h = 0; h < SUB; ++h)
+        for (int h = 0; h < SUB; ++h) {
+          if (h < nh) {
+            unsigned long long mine = 0;
 #pragma unroll
-          for (int r = 0; r < RPT; ++r) {
-            const int i2 = h * NT + cg * RPT + r;
-            if (i2 < ng) {
+            for (int r = 0; r < RPT; ++r) {
+              unsigned long long v;
               if (PASS == 0) {
                 const int m = __reduce_max_sync(0xffffffffu, mx[h][r]);
-                if (lane == 0 && m != INT32_MIN) atomicMax(w.rowmax + rowq[i2], tt_key(m));
+                v = m == INT32_MIN ? 0ull : tt_key(m);
               } else {                                       // 32 lanes x 63 units x 2^24 < 2^35: two halves
                 const uint32_t lo = __reduce_add_sync(0xffffffffu, es[h][r] & 0xffffu), hi = __reduce_add_sync(0xffffffffu, es[h][r] >> 16);
-                const unsigned long long s = lo + ((unsigned long long)hi << 16);
-                if (lane == 0 && s) atomicAdd(w.rowsum + rowq[i2], s);
+                v = lo + ((unsigned long long)hi << 16);
               }
+              mine = lane == r ? v : mine;
+            }
+            if (lane < RPT) {
+              if (PASS == 0) atomicMax(&row_sh[h * NT + cg * RPT + lane], mine);
+              else atomicAdd(&row_sh[h * NT + cg * RPT + lane], mine);
             }
           }
+        }
+        named_sync(1, TT_COMPUTE);
+        if (tid < ng && row_sh[tid]) {
+          if (PASS == 0) atomicMax(w.rowmax + rowq[tid], row_sh[tid]);
+          else atomicAdd(w.rowsum + rowq[tid], row_sh[tid]);
+        }
       } else {
         load_k(0);
         store_k(0);
@@ -693,12 +731,21 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
               tmem_ld4(tlane + cg * RPT + r0, ll);
               tmem_ld4(tlane + NT + cg * RPT + r0, md);
               tmem_ld4(tlane + 2 * NT + cg * RPT + r0, hh);
-              tmem_wait_ld();
+              tmem_wait12(ll, md, hh);
               if (mode == 0) {
 #pragma unroll
                 for (int f = 0; f < 4; ++f) {
                   const TtRow rc = rowc[cg * RPT + r0 + f];
                   const int sh = rc.qs + ksh, sc = high(sum64(ll[f], md[f], hh[f], sh), sh);
+                  pr[r0 + f] = prob_of(exp_sm_flat(T, (uint32_t)rc.base - (uint32_t)sc), ((uint64_t)rc.ihi << 32) | rc.ilo);
+                }
+              } else if (mode == 3) {
+#pragma unroll
+                for (int f = 0; f < 4; ++f) {
+                  const int i2 = cg * RPT + r0 + f;
+                  const TtRow rc = rowc[i2];
+                  const int sh = rc.qs + max(ksh, 0);
+                  const int sc = seen(i2, ksh, t) ? high(sum64(ll[f], md[f], hh[f], sh), sh) : INT32_MIN;
                   pr[r0 + f] = prob_of(exp_sm_flat(T, (uint32_t)rc.base - (uint32_t)sc), ((uint64_t)rc.ihi << 32) | rc.ilo);
                 }
               } else {
@@ -739,24 +786,29 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
         wait(&bar_p, ph_p, 0);
         __syncwarp();
         tc_fence_after();
-        // the run's sums: lane = dim, columns = rows
-        const int c = key % RS, dim = 4 * c + key / RS;
-        const bool has = key < 4 * RS && c < HD / 4;
+        // the run's sums: lane = dim, columns = rows; through shared memory (V's planes), so that a warp's
+        // atomics are of neighbouring dims
+        int64_t* stage = reinterpret_cast<int64_t*>(sm + G::OFF_V);          // [row][MMA row], 48 x 128
 #pragma unroll
         for (int r0 = 0; r0 < RPT; r0 += 4) {
           int v[6][4];
 #pragma unroll
           for (int s = 0; s < 6; ++s) tmem_ld4(tlane + G::ACC + s * NT + cg * RPT + r0, v[s]);
-          tmem_wait_ld();
+          tmem_wait12(v[0], v[1], v[2]);
+          tmem_wait12(v[3], v[4], v[5]);
 #pragma unroll
           for (int f = 0; f < 4; ++f) {
-            const int col = cg * RPT + r0 + f, i2 = (col & 3) * RPT + (col >> 2);
-            if (i2 < ng) {
-              int64_t o = mad_wide_s32(v[3][f], 1 << 24, mad_wide_s32(v[2][f], 1 << 16, mad_wide_s32(v[1][f], 256, (int64_t)v[0][f])));
-              o += (int64_t)(((uint64_t)(uint32_t)v[4][f] + ((uint64_t)(uint32_t)v[5][f] << 8)) << 32);
-              if (has && o) atomicAdd(reinterpret_cast<unsigned long long*>(a.out) + rowq[i2] * HD + dim, (unsigned long long)o);
-            }
+            int64_t o = mad_wide_s32(v[3][f], 1 << 24, mad_wide_s32(v[2][f], 1 << 16, mad_wide_s32(v[1][f], 256, (int64_t)v[0][f])));
+            o += (int64_t)(((uint64_t)(uint32_t)v[4][f] + ((uint64_t)(uint32_t)v[5][f] << 8)) << 32);
+            stage[(cg * RPT + r0 + f) * 128 + key] = o;
           }
+        }
+        tc_fence_before();
+        named_sync(1, TT_COMPUTE);
+        for (int e = tid; e < NT * HD; e += TT_COMPUTE) {
+          const int col = e / HD, dim = e - col * HD, i2 = (col & 3) * RPT + (col >> 2);
+          const int64_t o = stage[col * 128 + (dim & 3) * RS + (dim >> 2)];
+          if (i2 < ng && o) atomicAdd(reinterpret_cast<unsigned long long*>(a.out) + rowq[i2] * HD + dim, (unsigned long long)o);
         }
         tc_fence_before();
       }
