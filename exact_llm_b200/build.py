@@ -1,4 +1,5 @@
-"""Build the in-tree CUDA library libexactb200.so for sm_100a (nvcc, no torch dependency).
+"""Build the in-tree CUDA library libexactb200.so for sm_100a (nvcc, no torch dependency) and, beside it,
+libexactb200_torch.so (g++ and torch's headers): the torch operators that call it (torch_ops.cpp).
 
 Every .cu file compiles to its own object in parallel (whole-program device code per file, no
 relocatable device code: the translation units share only inline header code), then one nvcc
@@ -13,6 +14,8 @@ ROOT = os.path.dirname(HERE)
 SRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(ROOT, "_build")
 LIB = os.path.join(HERE, "libexactb200.so")
+TORCH_SRC = os.path.join(HERE, "torch_ops.cpp")
+TORCH_LIB = os.path.join(HERE, "libexactb200_torch.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
@@ -75,5 +78,34 @@ def build(force=False, verbose=False, extra=()):
     return LIB
 
 
+def build_torch(force=False, verbose=False):
+    """The torch operators.  Needs torch; without it there is nothing to register them with."""
+    try:
+        import torch
+        from torch.utils.cpp_extension import include_paths, library_paths
+    except ImportError:
+        print("torch is not installed: no torch operators")
+        return None
+    newest = max(os.path.getmtime(p) for p in (TORCH_SRC, os.path.join(ROOT, "include", "exactb200.h")))
+    if not force and os.path.exists(TORCH_LIB) and os.path.getmtime(TORCH_LIB) > newest:
+        return TORCH_LIB
+    import sysconfig
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    inc = include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda, "include"), os.path.join(ROOT, "include")]
+    libs = library_paths()
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-unknown-pragmas",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           "-o", TORCH_LIB + ".tmp", TORCH_SRC]
+    cmd += [x for i in inc for x in ("-isystem", i)]
+    cmd += [f"-L{d}" for d in libs] + ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
+    cmd += [f"-Wl,-rpath,{d}" for d in libs]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+    return TORCH_LIB
+
+
 if __name__ == "__main__":
     build(force="--force" in sys.argv, verbose=True, extra=[a for a in sys.argv[1:] if a != "--force"])
+    build_torch(force="--force" in sys.argv, verbose=True)

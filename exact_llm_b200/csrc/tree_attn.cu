@@ -488,26 +488,32 @@ static cudaError_t launch_cluster_hd(const TreeArgs& a, int C, int ldk, cudaStre
   }
 }
 
-// Many rows in a group and much work: the tensor-core kernels.
+// The tensor-core kernels from about 8 million scores of 128 dims on, with rows enough in a group to fill
+// their tiles.  Measured both ways (28 heads of 128, 4 groups; one tree of 16, 32, 64 nodes): after 2000
+// tokens 29, 45, 89 us here and 64, 73, 100 there; after 8000 tokens 76, 147, 289 here and 95, 128, 187
+// there; the same at half the width needs twice the scores.
 static bool use_tc(const TreeArgs& a) {
-  return (int64_t)a.R * a.rep >= 32ll * a.B && (int64_t)a.R * a.H * a.cap >= (1ll << 22);
+  return (int64_t)a.R * a.rep >= 24ll * a.B && (int64_t)a.R * a.H * a.kv.hd >= ((1ll << 30) + a.cap - 1) / a.cap;
 }
 
 static cudaError_t launch_tree_attention(const TreeArgs& a, void* workspace, cudaStream_t st) {
   // rows per tile: 16 where the trees have that many in a group
   const int NT = (int64_t)a.R * a.rep > 8ll * a.B ? 2 : 1, NR = 8 * NT;
-  // CTAs per cluster: as many as keep every cluster resident at once (two CTAs an SM, one with 16 rows
-  // or a long score array), each with 64 positions at least; more where the scores need the room
+  // CTAs per cluster: as many as keep every cluster resident at once, each with 64 positions at least; more
+  // where the scores need the room.  A GPU processing cluster's SMs bound what fits together: at one CTA an
+  // SM (16 rows, or a long score array) 14 clusters of 8, and a second round doubles the time (8 nodes of
+  // 28 heads after 2000 tokens: 16 clusters of 8 37 us, of 4 28 us)
   const int64_t clusters = std::max<int64_t>(a.B, ((int64_t)a.R * a.rep + NR - 1) / NR) * a.kv.KV;
   auto pitch = [&](int c) { return tree_pitch(((a.cap + c - 1) / c + 31) / 16 * 16); };
   auto smem_of = [&](int c) { return 41024 + (size_t)2048 * NR + (size_t)(NR + 2) * pitch(c) * 4; };
-  int C = 1;
-  while (C < 16 && (smem_of(C) > (size_t)TREE_SMEM_MAX ||
-                    ((int64_t)C * 64 < a.cap && clusters * 2 * C <= (NT == 2 || smem_of(2 * C) > 110 * 1024 ? 148 : 296))))
-    C *= 2;
-  const size_t smem = smem_of(C);
+  int C = 0;
+  for (int c = 1; c <= 16; c *= 2) {
+    if (smem_of(c) > (size_t)TREE_SMEM_MAX) continue;
+    const int slots = (NT == 2 || smem_of(c) > 110 * 1024 ? 112 : 256) / (c == 16 ? 2 : 1);
+    if (!C || ((int64_t)(c / 2) * 64 < a.cap && clusters * c <= slots)) C = c;
+  }
+  if (!C || use_tc(a)) return launch_tree_tc(a, workspace, st);
   const int ldk = pitch(C);
-  if (smem > (size_t)TREE_SMEM_MAX || use_tc(a)) return launch_tree_tc(a, workspace, st);
   return NT == 2 ? launch_cluster_hd<2>(a, C, ldk, st) : launch_cluster_hd<1>(a, C, ldk, st);
 }
 
