@@ -37,14 +37,15 @@ struct TreeGeo {
   static constexpr int KP = 8 / DG;                          // warps that share a dim group: key parts
   static constexpr int KS = HD < 32 ? 1 : HD / 32;           // 32-dim steps of a score
   static constexpr int OUT = KP * NR * HD;                   // partial outputs (int64)
-  // exp table, partial outputs, score rows, the V rows' places
-  static size_t smem(int ldk) { return 41024 + (size_t)OUT * 8 + (size_t)(NR + 2) * ldk * 4; }
+  // exp table, partial outputs, then per position: scores, the place of its V row (and of its K row where that
+  // is another number of elements), its shift
+  static size_t smem(int ldk, bool same) { return 41024 + (size_t)OUT * 8 + (size_t)ldk * (NR * 4 + (same ? 10 : 18)); }
 };
 // score row pitch for n positions: 4 mod 16 words, so a warp's stores and loads hit 32 banks
 inline int tree_pitch(int64_t n) { return (int)((n + 15) / 16 * 16 + 4); }
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(const TreeArgs a, int ldk) {
+__global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(const TreeArgs a, int ldk, bool same) {
   using G = TreeGeo<HD, NT>;
   constexpr int NR = G::NR;
   extern __shared__ __align__(128) unsigned char sm[];
@@ -52,6 +53,8 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
   int64_t* pout = reinterpret_cast<int64_t*>(sm + 41024);                    // KP x NR x HD
   int32_t* sc = reinterpret_cast<int32_t*>(sm + 41024 + (size_t)G::OUT * 8); // NR x ldk
   int64_t* vat = reinterpret_cast<int64_t*>(sc + (size_t)NR * ldk);          // V row of every position, in elements
+  int64_t* kat = same ? vat : vat + ldk;                                     // and K row
+  int16_t* ksh = reinterpret_cast<int16_t*>(kat + ldk);                      // its shift, -1: there is no such position
   __shared__ int64_t lmax[NR], lsum[NR];
   __shared__ int64_t wmax[8][NR];
   __shared__ uint64_t pinv[NR];
@@ -135,6 +138,27 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
   const int t0 = min(sq.S, c * chunk), n = min(sq.S, t0 + chunk) - t0;
   const int n32 = (n + 31) & ~31;
 
+  // ---- where the rows lie; all of them are on their way to L2 before the first is used
+  for (int t = tid; t < n32; t += TC_THREADS_T) {
+    int off = 0;
+    const int pg = t < n ? page_of(a, trow, t0 + t, off) : -1;
+    int64_t vo = 0, ko = 0;                                  // (a position that is not there: some row, hidden)
+    int sh = -1;
+    if (pg >= 0) {
+      const int16_t* kr = k_row(kv, j, pg, off);
+      const int32_t* vr = v_row(kv, j, pg, off);
+#pragma unroll
+      for (int o = 0; o < HD * 2; o += 128) prefetch_l2_line(reinterpret_cast<const char*>(kr) + o);
+#pragma unroll
+      for (int o = 0; o < HD * 4; o += 128) prefetch_l2_line(reinterpret_cast<const char*>(vr) + o);
+      sh = (uint8_t)k_shift(kv, j, pg, off);
+      ko = kr - kv.k;
+      vo = vr - kv.v;
+    }
+    vat[t] = vo;
+    if (!same) kat[t] = ko;
+    ksh[t] = (int16_t)sh;
+  }
   // ---- query digits: operand B of the scores; contraction slots 4 tq + i and 16 + 4 tq + i of a step
   // hold dims 8 tq + i and 8 tq + 4 + i, so that a key row is read 16 bytes at a time
   uint32_t ql[NT][G::KS][2], qh[NT][G::KS][2];
@@ -176,27 +200,15 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
     int4 k[2][G::KS];
     int sh[2];                                               // -1: no such key
   };
-  auto fetch = [&](int u, Keys& x, bool store) {
+  auto fetch = [&](int u, Keys& x) {
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
       const int t = u + g + 8 * f;
-      int off = 0;
-      const int pg = t < n ? page_of(a, trow, t0 + t, off) : -1;
-      x.sh[f] = -1;
+      const int16_t* kr = kv.k + kat[t] + 8 * tq;
+      x.sh[f] = ksh[t];
 #pragma unroll
-      for (int ks = 0; ks < G::KS; ++ks) x.k[f][ks] = make_int4(0, 0, 0, 0);
-      if (pg >= 0) {
-        const int16_t* kr = k_row(kv, j, pg, off);
-#pragma unroll
-        for (int ks = 0; ks < G::KS; ++ks)
-          if (ks * 32 + 8 * tq < HD) x.k[f][ks] = *reinterpret_cast<const int4*>(kr + ks * 32 + 8 * tq);
-        x.sh[f] = (uint8_t)k_shift(kv, j, pg, off);
-      }
-      if (store && tq == 0) {                                // V is needed after the exchanges: into L2 now
-        const int32_t* vr = v_row(kv, j, max(pg, 0), off);
-        if (pg >= 0) prefetch_l2_bulk(vr, HD * 4);
-        vat[t] = pg >= 0 ? vr - kv.v : 0;       // a key that is not there has p = 0
-      }
+      for (int ks = 0; ks < G::KS; ++ks)
+        x.k[f][ks] = ks * 32 + 8 * tq < HD ? __ldg(reinterpret_cast<const int4*>(kr + ks * 32)) : make_int4(0, 0, 0, 0);
     }
   };
   // one sweep over the keys: `wide` scores in 64 bits, `store` into sc
@@ -204,11 +216,11 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
     constexpr bool wide = decltype(wide_t)::value;
     bool fits = true;
     Keys next;
-    if (warp * 16 < n) fetch(warp * 16, next, store);
+    if (warp * 16 < n) fetch(warp * 16, next);
 #pragma unroll 1
     for (int u = warp * 16; u < n; u += 128) {
       const Keys x = next;
-      if (u + 128 < n) fetch(u + 128, next, store);
+      if (u + 128 < n) fetch(u + 128, next);
       const int sh[2] = {max(x.sh[0], 0), max(x.sh[1], 0)};
       if (!wide) fits &= sh[0] + qmax <= 13 && sh[1] + qmax <= 13;
       int ll[NT][4], md[NT][4], hh[NT][4];
@@ -301,10 +313,9 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
     cta_max();
   }
   // hidden rows of the tail, so that the loops below take whole steps of 32
-  for (int e = tid; e < (NR + 1) * (n32 - n); e += TC_THREADS_T) {
+  for (int e = tid; e < NR * (n32 - n); e += TC_THREADS_T) {
     const int i = e / (n32 - n), t = n + e - i * (n32 - n);
-    if (i < NR) sc[i * ldk + t] = INT32_MIN;
-    else vat[t] = 0;
+    sc[i * ldk + t] = INT32_MIN;
   }
   cluster.sync();
   // thread (row, peer): every peer's word at once, then over the C lanes of the row (C a power of two)
@@ -373,10 +384,13 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
         v[i] = __ldg(reinterpret_cast<const int4*>(vbase + vat[u + tq + 4 * i]));           // past the CTA's keys p is 0
       }
     };
+    // 16 rows: the next step's V rows are fetched a step ahead; 8 rows: two CTAs an SM hide them, and the
+    // registers that it takes would spill (32 single tokens after 1000: 55 us with it, 47 without)
     int4 v[8];
-    if (part * 32 < n) load_v(part * 32, v);
+    if (NT > 1 && part * 32 < n) load_v(part * 32, v);
 #pragma unroll 1
     for (int u = part * 32; u < n; u += 32 * G::KP) {
+      if (NT == 1) load_v(u, v);
       uint32_t va[2][4][4];                                  // tile, digit, fragment
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -389,7 +403,7 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
           for (int p = 0; p < 4; ++p) va[d >> 1][p][(d & 1) + 2 * h] = o[p];
         }
       }
-      if (u + 32 * G::KP < n) load_v(u + 32 * G::KP, v);
+      if (NT > 1 && u + 32 * G::KP < n) load_v(u + 32 * G::KP, v);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         uint32_t pb[2][4];                                   // half, digit
@@ -455,7 +469,7 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
 }
 
 template <int HD, int NT>
-static cudaError_t launch_cluster(const TreeArgs& a, int C, int ldk, cudaStream_t st) {
+static cudaError_t launch_cluster(const TreeArgs& a, int C, int ldk, bool same, cudaStream_t st) {
   using G = TreeGeo<HD, NT>;
   static DevOnce attr_set;
   if (!attr_set.done()) {
@@ -467,7 +481,7 @@ static cudaError_t launch_cluster(const TreeArgs& a, int C, int ldk, cudaStream_
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)C * (unsigned)((int64_t)a.R * a.rep / G::NR + a.B), a.kv.KV);
   cfg.blockDim = dim3(TC_THREADS_T);
-  cfg.dynamicSmemBytes = G::smem(ldk);
+  cfg.dynamicSmemBytes = G::smem(ldk, same);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -475,16 +489,16 @@ static cudaError_t launch_cluster(const TreeArgs& a, int C, int ldk, cudaStream_
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_tree_cluster<HD, NT>, a, ldk);
+  return cudaLaunchKernelEx(&cfg, k_tree_cluster<HD, NT>, a, ldk, same);
 }
 
 template <int NT>
-static cudaError_t launch_cluster_hd(const TreeArgs& a, int C, int ldk, cudaStream_t st) {
+static cudaError_t launch_cluster_hd(const TreeArgs& a, int C, int ldk, bool same, cudaStream_t st) {
   switch (a.kv.hd) {
-    case 16: return launch_cluster<16, NT>(a, C, ldk, st);
-    case 32: return launch_cluster<32, NT>(a, C, ldk, st);
-    case 64: return launch_cluster<64, NT>(a, C, ldk, st);
-    default: return launch_cluster<128, NT>(a, C, ldk, st);
+    case 16: return launch_cluster<16, NT>(a, C, ldk, same, st);
+    case 32: return launch_cluster<32, NT>(a, C, ldk, same, st);
+    case 64: return launch_cluster<64, NT>(a, C, ldk, same, st);
+    default: return launch_cluster<128, NT>(a, C, ldk, same, st);
   }
 }
 
@@ -505,7 +519,9 @@ static cudaError_t launch_tree_attention(const TreeArgs& a, void* workspace, cud
   // 28 heads after 2000 tokens: 16 clusters of 8 37 us, of 4 28 us)
   const int64_t clusters = std::max<int64_t>(a.B, ((int64_t)a.R * a.rep + NR - 1) / NR) * a.kv.KV;
   auto pitch = [&](int c) { return tree_pitch(((a.cap + c - 1) / c + 31) / 16 * 16); };
-  auto smem_of = [&](int c) { return 41024 + (size_t)2048 * NR + (size_t)(NR + 2) * pitch(c) * 4; };
+  const exb_kv_view& kv = a.kv;
+  const bool same = kv.k_page == kv.v_page && kv.k_head == kv.v_head && kv.k_pos == kv.v_pos;
+  auto smem_of = [&](int c) { return 41024 + (size_t)2048 * NR + (size_t)pitch(c) * (NR * 4 + (same ? 10 : 18)); };
   int C = 0;
   for (int c = 1; c <= 16; c *= 2) {
     if (smem_of(c) > (size_t)TREE_SMEM_MAX) continue;
@@ -514,7 +530,7 @@ static cudaError_t launch_tree_attention(const TreeArgs& a, void* workspace, cud
   }
   if (!C || use_tc(a)) return launch_tree_tc(a, workspace, st);
   const int ldk = pitch(C);
-  return NT == 2 ? launch_cluster_hd<2>(a, C, ldk, st) : launch_cluster_hd<1>(a, C, ldk, st);
+  return NT == 2 ? launch_cluster_hd<2>(a, C, ldk, same, st) : launch_cluster_hd<1>(a, C, ldk, same, st);
 }
 
 // what is wrong with a cache description, or nullptr

@@ -68,6 +68,8 @@ EXB_DEV int page_of(const TreeArgs& a, const int32_t* __restrict__ row, int pos,
   set_err(a.status, ERR_BOUNDS);
   return -1;
 }
+// the 128-byte line of an address into L2 (for rows of cache lines a third of the time of bulk prefetches)
+EXB_DEV void prefetch_l2_line(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p) : "memory"); }
 EXB_DEV const int16_t* k_row(const exb_kv_view& kv, int head, int pg, int off) {
   return kv.k + (int64_t)pg * kv.k_page + (int64_t)head * kv.k_head + (int64_t)off * kv.k_pos;
 }
