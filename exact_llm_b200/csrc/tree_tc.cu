@@ -11,10 +11,11 @@
 //               the whole run of units (at most 3 * 255^2 * 8064 positions < 2^31)
 //   digits      cache rows come through registers: K in 16-byte pieces, V in blocks of 4 positions x 4
 //               dims that byte permutations turn into words of 4 positions per digit
-//   warps       16 compute warps (TMEM lane = position, four column groups), three that issue the MMAs (one
-//               alone took 90 cycles an MMA next to the compute warps, twice what the tensor core takes) and
-//               one that looks up the pages; they meet on mbarriers only, so the look-ups, the loads, the
-//               digits, the MMAs and the softmax of neighbouring units overlap
+//   warps       16 that turn scores into maxima, sums or probabilities (TMEM lane = position, four column
+//               groups), 8 that load cache rows and make digits of them, 3 that issue the MMAs (one alone took 90
+//               cycles an MMA next to the others, twice what the tensor core takes) and one that looks up the
+//               pages; they meet on mbarriers only, so the look-ups, the loads, the digits, the MMAs and the
+//               softmax of neighbouring units overlap
 // Scores are computed anew in each kernel: keeping them would move 12 bytes a score, more than the MMAs
 // and the three multiply-adds that make one cost.
 #include <algorithm>
@@ -27,13 +28,16 @@
 
 namespace exb {
 
-constexpr int TT_CW = 16;                          // compute warps
+constexpr int TT_CW = 16;                          // softmax warps
 constexpr int TT_COMPUTE = 32 * TT_CW;
-constexpr int TT_THREADS = TT_COMPUTE + 128;       // and four: MMAs (two or three), places
+constexpr int TT_LW = 8;                           // loading warps
+constexpr int TT_LOAD = 32 * TT_LW;
+constexpr int TT_THREADS = TT_COMPUTE + TT_LOAD + 128;       // and four: MMAs (two or three), places
 constexpr int TT_BK = 128;                         // positions per unit
 constexpr int TT_CHUNK = 32;                       // a chunk is 32 to 63 units of positions (all, if fewer): its row
                                                    // tiles follow one another, so its cache rows are read from L2
                                                    // by all but the first; a run is a part of a chunk
+constexpr uint32_t TT_WAIT_LIMIT = 1u << 20;       // polls of a wait (a limit that depends on earlier waits costs 4%)
 constexpr int TT_RING = 8;                         // units whose rows' places are kept
 
 struct TtPlaces {                                  // where a unit's cache rows lie, in elements, and the shifts
@@ -193,9 +197,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
   constexpr int NT = G::NT, RPT = G::RPT, SUB = G::SUB;
   constexpr int KS = HD < 32 ? 1 : HD / 32;                  // 32-byte steps of a score
   constexpr int KCH = HD / 8;                                // 16-byte pieces of a key row
-  constexpr int KC = TT_BK * KCH >= TT_COMPUTE ? TT_BK * KCH / TT_COMPUTE : 1;
-  constexpr bool KALL = TT_BK * KCH >= TT_COMPUTE;
-  constexpr int VB = HD >= 128 ? 2 : 1;                      // V blocks (16 positions x 32 dims) a warp
+  constexpr int KC = TT_BK * KCH / TT_LOAD;                  // of a loading thread
+  constexpr int VB = HD >= 64 ? 2 : 1;                       // V blocks (16 positions x 32 dims) a warp loads at once
+  constexpr int VH = HD >= 128 ? 2 : 1;                      // and how often
   constexpr int RS = HD < 32 ? 8 : HD / 4;                   // dim 4 c + d is MMA row d RS + c
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -206,12 +210,15 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
   __shared__ int64_t rmax[PASS ? G::NR : 1];
   __shared__ int64_t rowq[G::NR];                            // row of q, qs and out
   __shared__ unsigned long long row_sh[PASS < 2 ? G::NR : 1];
-  // bar_s: a score tile is complete; bar_f: every warp has read it; bar_k: a unit's keys are in place (PASS 2:
-  // its P and V and the keys of the next but one); bar_q: a run's first keys (PASS 2); bar_p: the p . v
-  // products of a unit are complete.  A waiter never falls two phases behind: what comes two phases later
-  // depends on what it does after its wait.
-  // ring_full, ring_free: a unit's places are written, every warp is done with them
-  __shared__ uint64_t bar_s[2], bar_f[2], bar_k[2], bar_p, bar_q, ring_full[TT_RING], ring_free[TT_RING];
+  // Barriers by unit or tile number, two of a kind where the second to next depends on the wait for this one:
+  //   bar_s   a score tile is complete        bar_f   every softmax warp has read it
+  //   bar_k   a unit's keys are in place      bar_kf  its score MMAs are complete (the buffer is free)
+  //   bar_v   V is in place                   bar_w   P is in place
+  //   bar_p   the p . v products are complete
+  //   bar_q   a run's query digits are in place, and what the last run left in shared memory is used up
+  //           (two by turns as well: a warp that issues scores has no part in a run of one tile, but in the next)
+  //   ring_full, ring_free   a unit's places are written, every warp is done with them
+  __shared__ uint64_t bar_s[2], bar_f[2], bar_k[2], bar_kf[2], bar_v[2], bar_w[2], bar_p, bar_q[2], ring_full[TT_RING], ring_free[TT_RING];
   __shared__ uint32_t tmem_sh;
   __shared__ int qmax_sh;
   __shared__ volatile uint32_t top_sh[2];                    // the last unit (+ 1) with a third digit in some p
@@ -222,18 +229,21 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar_s[i], 1);
       mbar_init(&bar_f[i], TT_CW);
-      mbar_init(&bar_k[i], TT_CW);
+      mbar_init(&bar_k[i], TT_LW);
+      mbar_init(&bar_kf[i], PASS < 2 ? 2 : 1);               // two warps issue the scores of a unit's two tiles
+      mbar_init(&bar_v[i], TT_LW);
+      mbar_init(&bar_w[i], TT_CW);
+      mbar_init(&bar_q[i], TT_CW);
     }
     for (int i = 0; i < TT_RING; ++i) {
       mbar_init(&ring_full[i], 1);
-      mbar_init(&ring_free[i], TT_CW);
+      mbar_init(&ring_free[i], TT_CW + TT_LW);
     }
-    mbar_init(&bar_q, TT_CW);
     mbar_init(&bar_p, 2);                                    // two warps issue the products
     top_sh[0] = top_sh[1] = 0;
     mbar_fence_init();
   }
-  if (warp == TT_CW) {
+  if (warp == TT_CW + TT_LW) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_sh)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -252,19 +262,22 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
   int64_t u = total * blockIdx.x / gridDim.x;
   const int64_t uend = total * (blockIdx.x + 1) / gridDim.x;
   bool late = false;                                         // a wait gave up
-  // parity of the next completion of each barrier, as this thread waits for them
-  uint32_t ph_s = 0, ph_f = 0, ph_q = 0, ph_p = 0;           // bit i: barrier i
-  auto wait = [&](uint64_t* bar, uint32_t& ph, int i) {
-    late |= !mbar_wait(bar + i, (ph >> i) & 1, TC_WAIT_LIMIT);
-    ph ^= 1u << i;
+  uint32_t tiles = 0, units = 0, runs = 0;                   // of this CTA so far
+  // the n-th completion (from 0) of a barrier; once a wait has given up, none waits any more and the kernel ends
+  auto wait = [&](uint64_t* bar, uint32_t n) {
+    late |= !mbar_wait(bar, n & 1, TT_WAIT_LIMIT);
   };
-  uint32_t tiles = 0, units = 0;                             // of this CTA so far
-  auto wait_k = [&](uint32_t unit) { late |= !mbar_wait(&bar_k[unit & 1], (unit >> 1) & 1, TC_WAIT_LIMIT); };
+  auto wait2 = [&](uint64_t* bar, uint32_t n) { wait(bar + (n & 1), n >> 1); };          // one of two, by turns
+  auto arrive = [&](uint64_t* bar) {                         // this warp, after all its lanes
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  };
+  auto await_places = [&](uint32_t unit) { wait(&ring_full[unit % TT_RING], unit / TT_RING); };
 
-  // 640 threads start with 96 registers each, 61440 in all; 128 x 48 + 512 x 104 = 59392
-  if (warp >= TT_CW) {
+  // 896 threads start with 72 registers each, 64512 in all; 512 x 80 + 256 x 64 + 128 x 48 = 63488
+  if (warp >= TT_CW + TT_LW) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-    const int role = warp - TT_CW;
+    const int role = warp - TT_CW - TT_LW;
     if (role == 3) {
       // ---- places: four positions a lane; the pages of the next unit are looked up meanwhile
       const int32_t* trow = nullptr;
@@ -307,7 +320,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
           }
         }
         more = next_pages();
-        if (units >= TT_RING) late |= !mbar_wait(&ring_free[slot], ((units / TT_RING) & 1) ^ 1, TC_WAIT_LIMIT);
+        if (units >= TT_RING) wait(&ring_free[slot], units / TT_RING - 1);
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
           out.k[lane + 32 * f] = k[f];
@@ -344,36 +357,38 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
         const TtRun run = tt_run(a, pre, G::NR, u, uend);
         u += run.nk;
         if constexpr (PASS < 2) {
+          bool begun = false;
           const TreeSeq sq = tree_seq(a, run.b, false);
           const int nh = sq.T * a.rep - run.rt * G::NR > NT ? 2 : 1;
           for (int i = 0; i < run.nk; ++i, ++units) {
             for (int h = 0; h < nh; ++h, ++tiles) {
               const int s = tiles & 1;
               if (role != s) continue;
-              wait_k(units);
-              if (tiles >= 2) wait(bar_f, ph_f, s);
+              if (!begun) wait2(bar_q, runs);
+              begun = true;
+              wait2(bar_k, units);
+              if (tiles >= 2) wait2(bar_f, tiles - 2);
               tc_fence_after();
               issue_scores(h, units & 1, s * 3 * NT);
               tc_commit(&bar_s[s]);
+              tc_commit(&bar_kf[units & 1]);
+              if (nh == 1) tc_commit(&bar_kf[units & 1]);
             }
           }
         } else if (role == 0) {
-          wait(&bar_q, ph_q, 0);
-          tc_fence_after();
-          issue_scores(0, 0, 0);
-          tc_commit(&bar_s[0]);
+          wait2(bar_q, runs);
           for (int i = 0; i < run.nk; ++i, ++units) {
-            if (i > 0 && i + 1 < run.nk) wait_k(units - 1);  // the keys of unit i + 1
-            wait(bar_f, ph_f, 0);
-            if (i + 1 < run.nk) {
-              tc_fence_after();
-              issue_scores(0, (i + 1) & 1, 0);
-              tc_commit(&bar_s[0]);
-            }
+            wait2(bar_k, units);
+            if (i > 0) wait(&bar_f[0], units - 1);
+            tc_fence_after();
+            issue_scores(0, units & 1, 0);
+            tc_commit(&bar_s[0]);
+            tc_commit(&bar_kf[units & 1]);
           }
-        } else {
+        } else if (role < 3) {
           for (int i = 0; i < run.nk; ++i, ++units) {
-            wait_k(units);
+            wait2(bar_v, units);
+            wait2(bar_w, units);
             tc_fence_after();
             const bool add = i > 0;                          // the first unit's first product of a weight starts it
             const bool top = !add || top_sh[units & 1] == units + 1;
@@ -399,19 +414,100 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
             tc_commit(&bar_p);
           }
         }
+        ++runs;
       }
     }
     __syncwarp();
+  } else if (warp >= TT_CW) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    // ---- loading warps: a thread's pieces have fixed places in the planes
+    const int lt = tid - TT_COMPUTE, lw = warp - TT_CW;
+    const int kr = lt / KCH, kc = lt % KCH;                  // first key and piece, then KSTEP keys on
+    constexpr int KSTEP = TT_LOAD / KCH;
+    const uint32_t ka = sb + G::OFF_K + kr * 128 + (((kc >> 1) ^ (kr & 7)) << 4) + (kc & 1) * 8;
+    // V block: 16 positions (group lw), 32 dims; lane: 4 dims (piece vc), positions 4 aq ..
+    const int vc = lane & 7, aq = lane >> 3;
+    const uint32_t va = sb + G::OFF_V + vc * 128 + ((lw ^ vc) << 4) + aq * 4;
+    auto load_v = [&](const TtPlaces& p, int half, int4* x) {
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        const int4* at = reinterpret_cast<const int4*>(kv.v + p.v[lw * 16 + aq * 4 + f]) + vc + 16 * half;
+#pragma unroll
+        for (int n = 0; n < VB; ++n)
+          if (HD >= 32 || vc < HD / 4) x[4 * n + f] = __ldg(at + 8 * n);
+      }
+    };
+    auto store_v = [&](int half, const int4* x) {
+#pragma unroll
+      for (int n = 0; n < VB; ++n) {
+        if (HD >= 32 || vc < HD / 4) {
+          uint32_t o4[4][4];
+          byte_planes(x[4 * n].x, x[4 * n + 1].x, x[4 * n + 2].x, x[4 * n + 3].x, o4[0]);
+          byte_planes(x[4 * n].y, x[4 * n + 1].y, x[4 * n + 2].y, x[4 * n + 3].y, o4[1]);
+          byte_planes(x[4 * n].z, x[4 * n + 1].z, x[4 * n + 2].z, x[4 * n + 3].z, o4[2]);
+          byte_planes(x[4 * n].w, x[4 * n + 1].w, x[4 * n + 2].w, x[4 * n + 3].w, o4[3]);
+          const uint32_t d0 = va + (16 * half + 8 * n) * 128;
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int p = 0; p < 4; ++p) sts32(d0 + p * 16384 + d * RS * 128, o4[d][p]);
+        }
+      }
+    };
+    auto keys = [&](uint32_t n) {                            // of unit n
+      await_places(n);
+      const TtPlaces& p = ring[n % TT_RING];
+      int4 x[KC];
+#pragma unroll
+      for (int c = 0; c < KC; ++c) x[c] = __ldg(reinterpret_cast<const int4*>(kv.k + p.k[kr + c * KSTEP]) + kc);
+      if (n >= 2) wait2(bar_kf, n - 2);                      // the buffer's last scores
+      const uint32_t d = ka + (n & 1) * 2 * G::KB;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        uint2 lo, hi;
+        int16_digits(x[c], lo, hi);
+        sts64(d + c * KSTEP * 128, lo.x, lo.y);
+        sts64(d + G::KB + c * KSTEP * 128, hi.x, hi.y);
+      }
+      fence_async_smem();
+      arrive(&bar_k[n & 1]);
+    };
+    const uint32_t all = (uint32_t)(uend - u);
+    if constexpr (PASS < 2) {
+      for (; units < all; ++units) {
+        keys(units);
+        arrive(&ring_free[units % TT_RING]);
+      }
+    } else {
+      if (all) keys(0);
+      while (u < uend) {
+        const TtRun run = tt_run(a, pre, G::NR, u, uend);
+        u += run.nk;
+        for (int i = 0; i < run.nk; ++i, ++units) {
+          if (units + 1 < all) keys(units + 1);              // a unit ahead of V, which waits for the products
+          const TtPlaces& p = ring[units % TT_RING];
+          int4 x[VB * 4];
+          load_v(p, 0, x);
+          if (units) wait(&bar_p, units - 1);                // V's last products
+          if (i == 0) wait2(bar_q, runs);                    // and the last run's sums, which went through V's planes
+#pragma unroll
+          for (int half = 0; half < VH; ++half) {
+            if (half) load_v(p, half, x);
+            store_v(half, x);
+          }
+          fence_async_smem();
+          arrive(&bar_v[units & 1]);
+          arrive(&ring_free[units % TT_RING]);
+        }
+        ++runs;
+      }
+    }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 80;");
     const int quarter = warp & 3, cg = warp >> 2;            // TMEM lanes 32 quarter .., rows RPT cg ..
     const int key = quarter * 32 + lane;
     const uint32_t tlane = tmem + ((uint32_t)(quarter * 32) << 16);
     const int c2 = (int)(a.inv << 16), c1 = (int)(a.inv << 8), c0 = (int)a.inv;
-    auto arrive = [&](uint64_t* bar) {                       // this warp, after all its lanes
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
-    };
     while (u < uend) {
       const TtRun run = tt_run(a, pre, G::NR, u, uend);
       const TreeSeq sq = tree_seq(a, run.b, false);
@@ -459,66 +555,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
         rowc[tid] = r;
       }
 
-      // ---- cache rows through registers; a thread's pieces have fixed places in the planes
-      int4 kraw[KC];
-      int4 vraw[PASS == 2 ? VB * 4 : 1];
-      const int kr = tid / KCH, kc = tid % KCH;              // first key and piece, then KSTEP keys on
-      constexpr int KSTEP = TT_COMPUTE / KCH;
-      const uint32_t g = units;                              // the run's first unit
-      auto places = [&](int i) -> const TtPlaces& { return ring[(g + i) % TT_RING]; };
-      auto await_places = [&](int i) {
-        late |= !mbar_wait(&ring_full[(g + i) % TT_RING], ((g + i) / TT_RING) & 1, TC_WAIT_LIMIT);
-        __syncwarp();
-      };
-      auto load_k = [&](int i) {                             // (waits for the unit's places)
-        await_places(i);
-        const int64_t* p = places(i).k + kr;
-#pragma unroll
-        for (int c = 0; c < KC; ++c)
-          if (KALL || kr < TT_BK) kraw[c] = __ldg(reinterpret_cast<const int4*>(kv.k + p[c * KSTEP]) + kc);
-      };
-      const int ko = kr * 128 + (((kc >> 1) ^ (kr & 7)) << 4) + (kc & 1) * 8;
-      auto store_k = [&](int buf) {
-        const uint32_t d = sb + G::OFF_K + buf * 2 * G::KB + ko;
-#pragma unroll
-        for (int c = 0; c < KC; ++c)
-          if (KALL || kr < TT_BK) {
-            uint2 lo, hi;
-            int16_digits(kraw[c], lo, hi);
-            sts64(d + c * KSTEP * 128, lo.x, lo.y);
-            sts64(d + G::KB + c * KSTEP * 128, hi.x, hi.y);
-          }
-      };
-      // V block n of this warp: 16 positions kg, 32 dims; lane: 4 dims (piece vc), positions 4 aq ..
-      const int cl = lane & 7, aq = lane >> 3, kg = warp & 7, vc = (warp >> 3) * 8 + cl;
-      const uint32_t va = sb + G::OFF_V + vc * 128 + ((kg ^ (vc & 7)) << 4) + aq * 4;
-      auto load_v = [&](int i) {
-        const int64_t* p = places(i).v + kg * 16 + aq * 4;
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          const int4* at = reinterpret_cast<const int4*>(kv.v + p[f]) + vc;
-#pragma unroll
-          for (int n = 0; n < VB; ++n)
-            if (HD >= 64 || vc < HD / 4) vraw[4 * n + f] = __ldg(at + 16 * n);
-        }
-      };
-      auto store_v = [&]() {
-#pragma unroll
-        for (int n = 0; n < VB; ++n) {
-          if (HD >= 64 || vc < HD / 4) {
-            const int4 x0 = vraw[4 * n], x1 = vraw[4 * n + 1], x2 = vraw[4 * n + 2], x3 = vraw[4 * n + 3];
-            uint32_t o4[4][4];
-            byte_planes(x0.x, x1.x, x2.x, x3.x, o4[0]);
-            byte_planes(x0.y, x1.y, x2.y, x3.y, o4[1]);
-            byte_planes(x0.z, x1.z, x2.z, x3.z, o4[2]);
-            byte_planes(x0.w, x1.w, x2.w, x3.w, o4[3]);
-#pragma unroll
-            for (int d = 0; d < 4; ++d)
-#pragma unroll
-              for (int p = 0; p < 4; ++p) sts32(va + p * 16384 + (d * RS + 16 * n) * 128, o4[d][p]);
-          }
-        }
-      };
+      fence_async_smem();
+      named_sync(1, TT_COMPUTE);                             // query digits, rows and maxima are in place
+      arrive(&bar_q[runs & 1]);
+      ++runs;
+      const int qmax = qmax_sh;
       // ---- a score's sums put together, sh = qs + ks: n = 32 - sh, so the 64-bit sum shifted left by sh has the
       // score in its high words.  MODE 0: every position visible and sh in [0, 13], |score| < 2^31; MODE 3: the
       // same with the mask (a hidden score is INT32_MIN, 2^29 or more from any base); MODE 1: sh in [0, 31], with
@@ -561,22 +602,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
         for (int h = 0; h < SUB; ++h)
 #pragma unroll
           for (int r = 0; r < RPT; ++r) { mx[h][r] = INT32_MIN; es[h][r] = 0; }
-        load_k(0);
-        store_k(units & 1);
-        fence_async_smem();
-        named_sync(1, TT_COMPUTE);                           // query digits, rows and maxima are in place
-        arrive(&bar_k[units & 1]);
-        if (nk > 1) {
-          load_k(1);
-          store_k((units + 1) & 1);
-          fence_async_smem();
-          arrive(&bar_k[(units + 1) & 1]);
-        }
-        if (nk > 2) load_k(2);
-        const int qmax = qmax_sh;
 #pragma unroll 1
         for (int i = 0; i < nk; ++i, ++units) {
-          const int ksh = places(i).s[key];                  // shift of this thread's key; -1: no such position
+          await_places(units);
+          const int ksh = ring[units % TT_RING].s[key];      // shift of this thread's key; -1: no such position
           const int t = (kt0 + i) * TT_BK + key;
           const int mode = mode_of(ksh, t, qmax);
 #pragma unroll
@@ -584,7 +613,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
             if (h < nh) {
               const int s = tiles & 1;
               const int live = max(0, min(RPT, ng - h * NT - cg * RPT));          // this thread's rows that exist
-              wait(bar_s, ph_s, s);
+              wait2(bar_s, tiles);
               __syncwarp();
               tc_fence_after();
               const uint32_t col = tlane + s * 3 * NT + cg * RPT;
@@ -662,12 +691,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
               ++tiles;
             }
           }
-          if (i + 2 < nk) {                                  // the unit's keys are read: the next but one in their place
-            store_k(units & 1);
-            fence_async_smem();
-            arrive(&bar_k[units & 1]);
-            if (i + 3 < nk) load_k(i + 3);
-          }
           arrive(&ring_free[units % TT_RING]);
         }
         // the run's maxima and sums: over the warp's keys, lane r of a warp keeping row r's, over the four warps
@@ -702,26 +725,18 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
           else atomicAdd(w.rowsum + rowq[tid], row_sh[tid]);
         }
       } else {
-        load_k(0);
-        store_k(0);
-        if (nk > 1) { load_k(1); store_k(1); }
-        fence_async_smem();
-        named_sync(1, TT_COMPUTE);
-        arrive(&bar_q);
-        load_v(0);
-        if (nk > 2) load_k(2);
-        const int qmax = qmax_sh;
         const int live = max(0, min(RPT, ng - cg * RPT));    // this thread's rows that exist
         // row r of column group cg is row 4 r + cg of the P planes: two places of the key in them
         const uint32_t p0 = sb + G::OFF_P + cg * 128 + (((key >> 4) ^ cg) << 4) + (key & 15);
         const uint32_t p1 = sb + G::OFF_P + cg * 128 + (((key >> 4) ^ (4 + cg)) << 4) + (key & 15);
 #pragma unroll 1
         for (int i = 0; i < nk; ++i, ++units) {
-          const int ksh = places(i).s[key];                  // shift of this thread's key; -1: no such position
+          await_places(units);
+          const int ksh = ring[units % TT_RING].s[key];      // shift of this thread's key; -1: no such position
           const int t = (kt0 + i) * TT_BK + key;
           const int mode = mode_of(ksh, t, qmax);
           uint32_t pr[RPT];                                  // p of this key for the thread's rows
-          wait(bar_s, ph_s, 0);
+          wait(&bar_s[0], units);
           __syncwarp();
           tc_fence_after();
 #pragma unroll
@@ -762,7 +777,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
           }
           tc_fence_before();
           arrive(&bar_f[0]);                                 // the next unit's scores may come
-          if (i > 0) wait(&bar_p, ph_p, 0);                  // V, P and the other key buffer are free
+          if (units) wait(&bar_p, units - 1);                // P's planes are free
           uint32_t big = 0;
 #pragma unroll
           for (int r = 0; r < RPT; ++r) {
@@ -775,15 +790,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
             }
           }
           if (__any_sync(0xffffffffu, big >> 16) && lane == 0) top_sh[units & 1] = units + 1;
-          store_v();
-          if (i + 2 < nk) store_k(i & 1);
           fence_async_smem();
-          arrive(&bar_k[units & 1]);
-          if (i + 1 < nk) load_v(i + 1);
-          if (i + 3 < nk) load_k(i + 3);
+          arrive(&bar_w[units & 1]);
           arrive(&ring_free[units % TT_RING]);
         }
-        wait(&bar_p, ph_p, 0);
+        wait(&bar_p, units - 1);
         __syncwarp();
         tc_fence_after();
         // the run's sums: lane = dim, columns = rows; through shared memory (V's planes), so that a warp's
@@ -816,7 +827,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
   }
   if (late) set_err(a.status, ERR_WAIT_TIMEOUT);
   __syncthreads();
-  if (warp == TT_CW)
+  if (warp == TT_CW + TT_LW)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 

@@ -134,7 +134,8 @@ int exb_tree_attention(const exb_kv_view* kv, const int16_t* q, const int32_t* q
  *   tokens, parent int32 (R): the drafted token of every row and its parent's index in the sequence
  *     (a row never follows one that is not before it: parent < own index; -1 for node 0)
  *   path, out_tokens int32 (B, max_len): the accepted nodes (node 0 first) and the target's token at
- *     each, -1 past the end; n int32 (B): their number, at most max_len.  The last token is new. */
+ *     each, -1 past the end; n int32 (B): their number, at most max_len.  The last token is new.
+ *   exp_t as in exb_tree_attention, 16-byte aligned; tnum in [1, 2^32] */
 int exb_tree_verify(const int64_t* logits, int64_t ld, int R, int V, const int32_t* u20, int64_t tnum,
                     const int32_t* tokens, const int32_t* parent, const int32_t* row_start, int B, int max_len,
                     const int32_t* exp_t, int32_t* sampled, int32_t* n, int32_t* path, int32_t* out_tokens,
@@ -142,7 +143,8 @@ int exb_tree_verify(const int64_t* logits, int64_t ld, int R, int V, const int32
 
 /* Keep the accepted path of every sequence: row ctx[b] + path[b][j] moves to ctx[b] + j for j < n[b],
  * in every layer (path strictly increasing, as exb_tree_verify gives it; ld_path its row stride), and
- * new_ctx[b] = ctx[b] + n[b].  A malformed path leaves its sequence as it was (new_ctx[b] = ctx[b]).
+ * new_ctx[b] = ctx[b] + n[b] (another array than ctx).  A malformed path leaves its sequence as it was
+ * (new_ctx[b] = ctx[b]).
  * The pages written must belong to one sequence only. */
 int exb_kv_compact(const exb_kv_view* kv, const int32_t* table, int B, int max_pages, const int32_t* ctx,
                    const int32_t* path, int ld_path, const int32_t* n, int32_t* new_ctx, int32_t* status, void* stream);

@@ -217,6 +217,22 @@ def test_attention_random(gpu, exp_t, seed, wide):
 
 @pytest.mark.gpu
 @WIDE
+@pytest.mark.parametrize("seed", range(4))
+def test_attention_many_short_sequences(gpu, exp_t, seed, wide):
+    """More sequences than SMs, of a few hundred positions at most and trees of all sizes: every CTA goes through
+    several short pieces of work."""
+    rng = np.random.default_rng(50 + seed)
+    B = 250
+    nodes = rng.integers(1, [5, 30, 40, 64][seed], B)
+    ctx = rng.integers(0, [100, 300, 200, 100][seed], B)
+    p = ref.problem(seed, H=8, KV=2, hd=[64, 32, 128, 16][seed], page=16, ctx=[int(x) for x in ctx], nodes=[int(x) for x in nodes])
+    want = ref.attention(**p)
+    for _ in range(3):
+        assert np.array_equal(_attend(gpu, exp_t, p, None, wide).cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+@WIDE
 def test_attention_masks(gpu, exp_t, wide):
     """Rows that see nothing give zeros; bits past the tree count for nothing; any set of nodes will do."""
     p = ref.problem(5, H=6, KV=2, hd=64, page=16, ctx=[0, 20], nodes=[9, 70], words=3)
@@ -252,7 +268,7 @@ def test_attention_strides(gpu, exp_t, wide):
     torch = gpu
     p = ref.problem(7, H=10, KV=2, hd=64, page=48, ctx=[100, 30], nodes=[7, 20])
     want = ref.attention(**p)
-    for how in ("layer", "positions first", "padded"):
+    for how in ("layer", "positions first", "padded", "keys padded", "values padded"):
         new = {}
         for n in ("k", "ks", "v"):
             x = _dev(torch, p[n])
@@ -260,11 +276,30 @@ def test_attention_strides(gpu, exp_t, wide):
                 new[n] = torch.stack([x.roll(1, 0), x, x.roll(2, 0)])[1]
             elif how == "positions first":
                 new[n] = x.transpose(1, 2).contiguous().transpose(1, 2)
-            elif n != "ks":
+            elif n in {"padded": "kv", "keys padded": "k", "values padded": "v"}[how]:
                 pad = torch.full((*x.shape[:-1], x.shape[-1] + 8), -7, dtype=x.dtype, device="cuda")
                 pad[..., :x.shape[-1]] = x
                 new[n] = pad[..., :x.shape[-1]]
         assert np.array_equal(_attend(torch, exp_t, p, None, wide, **new).cpu().numpy(), want), how
+
+
+def _far(torch, x, pages):
+    """The array with its pages (axis `pages`) more than 2^29 elements apart: offsets past 32 bits."""
+    stride, at = [0] * x.ndim, 1
+    for i in [i for i in reversed(range(x.ndim)) if i != pages]:
+        stride[i], at = at, at * x.shape[i]
+    stride[pages] = (1 << 29) + 64
+    assert at <= stride[pages] and x.shape[pages] * stride[pages] > 1 << 31
+    far = torch.empty_strided(x.shape, stride, dtype=_dev(torch, x[:0]).dtype, device="cuda")
+    return far.copy_(_dev(torch, x))
+
+
+@pytest.mark.gpu
+@WIDE
+def test_attention_far_pages(gpu, exp_t, wide):
+    p = ref.problem(11, H=6, KV=2, hd=64, page=16, ctx=[50, 3], nodes=[7, 20])
+    far = {n: _far(gpu, p[n], 0) for n in ("k", "v")}
+    assert np.array_equal(_attend(gpu, exp_t, p, None, wide, **far).cpu().numpy(), ref.attention(**p))
 
 
 @pytest.mark.gpu
@@ -379,6 +414,18 @@ def test_verify(gpu, exp_t, V):
 @pytest.mark.parametrize("V", [151936, 152064, 262147])
 def test_verify_vocabularies(gpu, exp_t, V):
     p = _verify_problem(V, V, [4, 9])
+    assert _same(_verify(gpu, exp_t, p), ref.verify(**p))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,tnum", [(327680, 1 << 16), (327681, 1 << 16), (400001, 81920), (5000, (1 << 31) - 1),
+                                    (5000, 1 << 31), (5000, 1 << 32)])
+def test_verify_any_length_any_temperature(gpu, exp_t, V, tnum):
+    """Either side of what the clusters hold in registers, and of what their 32-bit products can scale."""
+    p = _verify_problem(V, V, [3, 2], spread=2.5 * (1 << 16) / tnum, tnum=tnum)
+    assert _same(_verify(gpu, exp_t, p), ref.verify(**p))
+    for i in range(5):                                       # scaled logits around 2^30
+        p["logits"][i] = np.random.default_rng(i).integers(-3, 3, V) + (((1 << 46) // tnum) + 1 if i % 2 else -((1 << 46) // tnum))
     assert _same(_verify(gpu, exp_t, p), ref.verify(**p))
 
 
@@ -533,6 +580,25 @@ def test_cache_strides(gpu):
     torch.ops.exact.kv_copy_pages_(*dev, *[_dev(torch, np.array([x], np.int32)) for x in (table[0, 1], free[0], 5)])
     for y in want:
         y[:, free[0], :, :5] = y[:, table[0, 1], :, :5]
+    assert all(np.array_equal(a.cpu().numpy(), b) for a, b in zip(dev, want))
+
+
+@pytest.mark.gpu
+def test_cache_far_pages(gpu):
+    """Pages more than 2^29 elements apart."""
+    torch = gpu
+    rng = np.random.default_rng(3)
+    table, pool = ref.paged(rng, [40], 16)
+    cache = [rng.integers(-9, 9, (2, pool, 2, 16, 32)).astype(np.int16), rng.integers(0, 9, (2, pool, 2, 16)).astype(np.int8),
+             rng.integers(-9, 9, (2, pool, 2, 16, 32)).astype(np.int32)]
+    path, n, ctx = np.array([[1, 4, 11]], np.int32), np.array([3], np.int32), np.array([20], np.int32)
+    dev = [_far(torch, cache[0], 1), _dev(torch, cache[1]), _far(torch, cache[2], 1)]
+    torch.ops.exact.kv_compact_(*dev, _dev(torch, table), _dev(torch, ctx), _dev(torch, path), _dev(torch, n))
+    want, _ = ref.compact(cache, table, ctx, path, n)
+    free = [i for i in range(pool) if i not in table][0]
+    torch.ops.exact.kv_copy_pages_(*dev, *[_dev(torch, np.array([x], np.int32)) for x in (table[0, 1], free, 5)])
+    for y in want:
+        y[:, free, :, :5] = y[:, table[0, 1], :, :5]
     assert all(np.array_equal(a.cpu().numpy(), b) for a, b in zip(dev, want))
 
 
