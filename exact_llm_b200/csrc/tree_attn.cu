@@ -4,7 +4,14 @@
 //   e_t = exp table at (max s - s_t), Q24;  p_t = (e_t << 20) // sum(e);  out = shr(sum p_t v_t, 20)
 //
 // p needs the row's final maximum and sum (a floor division by the sum: no rescaling afterwards
-// gives the same bits), so a row goes over its positions three times.
+// gives the same bits), so a row goes over its scores three times.  Here the scores stay in shared memory
+// meanwhile; tree_tc.cu computes them anew each time, for many rows and long caches.
+//
+// Measured on one B200 (device time in a graph): 32 single tokens of 28 heads after up to 1000 tokens 28.5 us
+// (11.4 us would be the 75 MB at the rate of a copy; every SM reads rows of 256 and 512 bytes by look-up, and
+// what it has in flight covers the latency of L2 and HBM in part); a tree of 26 nodes of 28 heads after 513
+// tokens 21.7 us and one token of an empty sequence 9.6 us (cluster barriers and the chain from the lengths
+// over the table to the rows: no bytes to speak of).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -502,12 +509,15 @@ static cudaError_t launch_cluster_hd(const TreeArgs& a, int C, int ldk, bool sam
   }
 }
 
-// The tensor-core kernels from about 8 million scores of 128 dims on, with rows enough in a group to fill
+// The tensor-core kernels from about 7 million scores of 128 dims on, with rows enough in a group to fill
 // their tiles.  Measured both ways (28 heads of 128, 4 groups; one tree of 16, 32, 64 nodes): after 2000
-// tokens 29, 45, 89 us here and 64, 73, 100 there; after 8000 tokens 76, 147, 289 here and 95, 128, 187
-// there; the same at half the width needs twice the scores.
+// tokens 28, 43, 83 us here and 61, 72, 97 there; after 8000 tokens 68, 129, 254 here and 91, 120, 179
+// there; 8 trees of 16 nodes of 40 heads, 8 groups, after 1000, 2000, 4000 tokens 78, 147, 239 and 99, 145,
+// 212; at half the width it takes twice the scores (64 nodes of 14 heads after 8000, 16000 tokens: 90, 176
+// and 110, 164).  With fewer than 24 rows a group most of a tile is empty (8 trees of 4 nodes of 28 heads after
+// 16000 tokens: 263 and 270).
 static bool use_tc(const TreeArgs& a) {
-  return (int64_t)a.R * a.rep >= 24ll * a.B && (int64_t)a.R * a.H * a.kv.hd >= ((1ll << 30) + a.cap - 1) / a.cap;
+  return (int64_t)a.R * a.rep >= 24ll * a.B && (int64_t)a.R * a.H * a.kv.hd >= ((7ll << 27) + a.cap - 1) / a.cap;
 }
 
 static cudaError_t launch_tree_attention(const TreeArgs& a, void* workspace, cudaStream_t st) {

@@ -18,6 +18,13 @@
 //               softmax of neighbouring units overlap
 // Scores are computed anew in each kernel: keeping them would move 12 bytes a score, more than the MMAs
 // and the three multiply-adds that make one cost.
+//
+// Measured on one B200 (device time in a graph): a tree of 61 nodes of 40 heads after 32768 tokens 791 us,
+// 24 digit products of 128 dims a score, 0.62 POP/s; 8 trees of up to 63 nodes of 28 heads after up to 4097
+// tokens 476 us.  A unit of the third kernel takes about 9000 cycles: 17 thousand warp instructions (the
+// exact exp table with its interpolation, the division by the sum, byte digits) at 2.1 a cycle, and of the
+// shared memory's cycles 4400 for their loads and stores (1900 are conflicts of the table's random look-ups)
+// and 2800 for the MMAs' operands; the tensor cores are busy a sixth of the time.
 #include <algorithm>
 #include <type_traits>
 
