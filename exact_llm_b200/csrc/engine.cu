@@ -1754,7 +1754,7 @@ int exb_tree_step(exb_model* m, int B, const int32_t* seqs, const int32_t* row_s
   if (!m->t_arena) {
     m->t_ws = all_bytes;
     m->t_ws_bytes = exb_tree_attention_workspace_bytes(PCH, c.H, c.max_batch);
-    CK(cudaMallocHost(&m->t_host, all_bytes));
+    if (!m->t_host) CK(cudaMallocHost(&m->t_host, all_bytes));
     CK(cudaMalloc(&m->t_arena, all_bytes + m->t_ws_bytes));
   }
   char *h = m->t_host, *d = m->t_arena;
