@@ -1717,6 +1717,8 @@ int exb_tree_step(exb_model* m, int B, const int32_t* seqs, const int32_t* row_s
     FAIL(EXB_EINVAL, "exb_tree_step: 1 <= B <= max_batch and no null argument");
   const int R = row_start[B];
   if (row_start[0] != 0 || R < 1 || R > chunk_rows(m)) FAIL(EXB_EINVAL, "exb_tree_step: 1 to 512 rows (256 for MoE) from row_start[0] = 0");
+  for (int b = 0; b < B; ++b)                                // (all of it before a node is looked at: R bounds what follows)
+    if (row_start[b + 1] < row_start[b] || row_start[b + 1] > R) FAIL(EXB_EINVAL, "exb_tree_step: row_start must rise");
   if (max_len < 1 || max_len > PCH) FAIL(EXB_EINVAL, "exb_tree_step: 1 <= max_len <= 512");
   if (tnum < 1 || tnum > (1ll << 32)) FAIL(EXB_EINVAL, "exb_tree_step: temperature multiplier in [1, 2^32]");
   std::vector<char> taken(c.max_batch, 0);

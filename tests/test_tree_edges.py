@@ -1,0 +1,26 @@
+"""Edges of the drafted-tree operators and of the engine's step on trees: sums, scores and random numbers at
+the ends of their ranges, malformed row ranges and arguments."""
+import ctypes
+
+import numpy as np
+import pytest
+
+
+# ------------------------------------------------------------------------------------------ the engine's step
+@pytest.mark.gpu
+@pytest.mark.parametrize("starts", [[0, 300, 5], [0, -1, 5], [0, 4, 3, 5], [0, 5, 2, 5], [0, 2**31 - 1, 5]])
+def test_tree_step_row_ranges(cuda_ok, starts):
+    """A row_start that falls, or leaves the rows in between, is refused before any node is read or kept: the arrays
+    passed hold the last entry's rows and no more."""
+    from exact_llm_b200._lib import lib
+    from tests.test_tree_decode import SMALL, _model, _prompt
+    m = _model(SMALL, max_batch=4, max_seq=400)
+    for s in range(3):
+        m.forward(_prompt(SMALL, 3), m.new_cache(s))
+    B, R = len(starts) - 1, starts[-1]
+    arr = [np.ascontiguousarray(x, np.int32) for x in
+           (range(B), starts, [1] * R, [-1] + list(range(R - 1)), np.zeros(B), np.zeros(B * 4), np.zeros(B * 4))]
+    seqs, rs, ids, par, n, path, tok = [x.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)) for x in arr]
+    rc = lib.exb_tree_step(m.h, B, seqs, rs, ids, par, None, 1 << 16, 4, n, path, tok, None, None)
+    assert rc == 1 and "row_start must rise" in lib.exb_last_error().decode()
+    assert [lib.exb_seq_len(m.h, s) for s in range(3)] == [3, 3, 3]
