@@ -661,7 +661,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
                       const bool see = seen(i2, ksh, t);
                       const int64_t sc = score64(M1{}, ll[f], md[f], hh[f], rowc[i2].qs + max(ksh, 0));
                       if (PASS == 0) {
-                        const bool fits = sc == (int)sc;
+                        const bool fits = sc == (int)sc && (int)sc != INT32_MIN;     // (INT32_MIN: nothing seen)
                         far |= see && !fits;                 // (its row is done anew below)
                         if (see && fits) mx[h][r0 + f] = max(mx[h][r0 + f], (int)sc);
                       } else if (see) {

@@ -5,6 +5,24 @@ import ctypes
 import numpy as np
 import pytest
 
+from tests import tree_ref as ref
+from tests.test_tree_ops import WIDE, _attend, exp_t, gpu  # noqa: F401
+
+
+# ------------------------------------------------------------------------------------------ attention
+@pytest.mark.gpu
+@WIDE
+@pytest.mark.parametrize("below", [0, 16])
+def test_attention_lowest_32_bit_score(gpu, exp_t, wide, below):  # noqa: F811
+    """A row whose largest score is -2^31 exactly sees its positions all the same."""
+    p = ref.problem(12, H=4, KV=2, hd=64, page=32, ctx=[300], nodes=[5])
+    p["q"][:], p["k"][:] = -16384, 16384 + below             # q.k = -2^34: times 2^13, shifted by 16
+    p["k"][p["table"][0, 0]] = 16384
+    p["qs"][:], p["ks"][:] = 9, 7
+    want = ref.attention(**p)
+    assert want.any()
+    assert np.array_equal(_attend(gpu, exp_t, p, None, wide).cpu().numpy(), want)
+
 
 # ------------------------------------------------------------------------------------------ the engine's step
 @pytest.mark.gpu
