@@ -237,11 +237,6 @@ __global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(con
   }
   __syncthreads();
   const uint64_t inv = linv;
-  if (!inv) {                                                 // a sum past the reciprocal's range
-    if (c == 0) sample_row<TV_THREADS>(a, r);
-    cluster.sync();
-    return;
-  }
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
     uint32_t p = 0;

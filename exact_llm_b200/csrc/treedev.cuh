@@ -80,12 +80,27 @@ EXB_DEV int k_shift(const exb_kv_view& kv, int head, int pg, int off) {
   return kv.ks[(int64_t)pg * kv.s_page + (int64_t)head * kv.s_head + (int64_t)off * kv.s_pos];
 }
 
-// p = (e << 20) // sum for 0 <= e <= 2^24 by two multiplications: inv = ceil(2^86 / sum), and
-// e * (inv * sum - 2^86) < 2^24 * 2^42 = 2^66, so (e * inv) >> 66 is the exact quotient for
-// 2^24 <= sum < 2^42: the row's largest term alone is 2^24 (entry 0 of the table), and 2^18 terms stay
-// below 2^42.  Other sums: 0.
+// p = (e << 20) // sum for 0 <= e <= 2^24 by two multiplications, p = (e * inv) >> 66.  The row's largest term
+// alone is 2^24 (entry 0 of the table), so a smaller sum is a row that sees nothing: inv = 0 and p = 0.
+//   2^24 <= sum < 2^42 (up to 2^18 terms): inv = ceil(2^86 / sum); e * (inv * sum - 2^86) < 2^24 * 2^42 = 2^66
+//     keeps the quotient exact
+//   sum >= 2^42: p is at most 4, the number of j in 1..4 with e >= t_j = ceil(j * sum / 2^20).  inv is the largest
+//     ceil(j * 2^66 / t_j): no smaller one takes t_j to j, and t_j - 1 stays below j, since 2^86 / sum lies between
+//     all j * 2^66 / t_j and all j * 2^66 / (t_j - 1), and two such fractions that differ are 2^18 apart or more
+EXB_DEV uint64_t prob_inverse_long(uint64_t sum) {
+  uint64_t inv = 0;
+#pragma unroll 1
+  for (uint64_t j = 1; j <= 4; ++j) {
+    const uint64_t t = (j * sum + (1u << 20) - 1) >> 20;
+    if (t > (1ull << 24)) break;
+    const uint64_t q = (j << 60) / t, r = (j << 60) - q * t;
+    inv = max(inv, (q << 6) + ((r << 6) + t - 1) / t);
+  }
+  return inv;
+}
 EXB_DEV uint64_t prob_inverse(uint64_t sum) {
-  if (sum < (1ull << 24) || sum >= (1ull << 42)) return 0;
+  if (sum < (1ull << 24)) return 0;
+  if (sum >= (1ull << 42)) return prob_inverse_long(sum);
   // a double's estimate is within 2^10 of the quotient (below 2^62 + 1), so the remainder 2^86 - q sum is
   // below 2^53 and its low 64 bits are all of it; the second estimate is within one of the rest
   const double rc = __drcp_rn((double)sum);

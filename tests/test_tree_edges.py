@@ -6,10 +6,31 @@ import numpy as np
 import pytest
 
 from tests import tree_ref as ref
-from tests.test_tree_ops import WIDE, _attend, exp_t, gpu  # noqa: F401
+from tests.test_tree_ops import WIDE, _attend, _same, _verify, _verify_problem, exp_t, gpu  # noqa: F401
 
 
 # ------------------------------------------------------------------------------------------ attention
+@pytest.mark.gpu
+@pytest.mark.parametrize("positions", [(1 << 18) - 1, 1 << 18, (1 << 18) + 1, 349526, 1 << 19, (1 << 20) + 1])
+def test_attention_flat_rows_of_long_caches(gpu, exp_t, positions):  # noqa: F811
+    """2^18 equal scores and more: the row's sum is 2^42 or more and a probability at most 4."""
+    p = ref.problem(positions, H=1, KV=1, hd=16, page=4096, ctx=[positions - 1], nodes=[1], vscale=2.0**13)
+    p["q"][:] = 0
+    want = ref.attention(**p)
+    assert want.any() == (positions <= 1 << 20)
+    assert np.array_equal(_attend(gpu, exp_t, p).cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("positions,qscale", [(400000, 0.02), (700001, 0.1), (1500000, 0.3)])
+def test_attention_small_probabilities(gpu, exp_t, positions, qscale):  # noqa: F811
+    """The same with scores of a small spread: probabilities of 0 to 4 side by side, two heads a group."""
+    p = ref.problem(positions, H=2, KV=1, hd=16, page=1024, ctx=[positions - 3], nodes=[3], qscale=qscale, vscale=2.0**13)
+    want = ref.attention(**p)
+    assert want.any()
+    assert np.array_equal(_attend(gpu, exp_t, p).cpu().numpy(), want)
+
+
 @pytest.mark.gpu
 @WIDE
 @pytest.mark.parametrize("below", [0, 16])
@@ -22,6 +43,17 @@ def test_attention_lowest_32_bit_score(gpu, exp_t, wide, below):  # noqa: F811
     want = ref.attention(**p)
     assert want.any()
     assert np.array_equal(_attend(gpu, exp_t, p, None, wide).cpu().numpy(), want)
+
+
+# ------------------------------------------------------------------------------------------ verification
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [262143, 262144, 262145, 327680])
+def test_verify_flat_rows(gpu, exp_t, V):  # noqa: F811
+    """Equal logits of 2^18 entries and more: sums around 2^42."""
+    p = _verify_problem(1, V, [5], greedy=0.0)
+    p["logits"][:4] = 12345
+    p["u20"][:] = [0, 1, (1 << 20) - 1, 1 << 19, 77]
+    assert _same(_verify(gpu, exp_t, p), ref.verify(**p))
 
 
 # ------------------------------------------------------------------------------------------ the engine's step
