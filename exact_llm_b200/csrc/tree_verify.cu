@@ -2,7 +2,8 @@
 // given random number or as the argmax, then the walk along the drafted tokens that agree.
 //
 //   y = shr(logit * tnum, 16), p = (e << 20) // sum(e) with e the exp table at (max y - y),
-//   token = first index whose running sum of p exceeds (u20 * sum(p)) >> 20     (exact_llm.py:243-259)
+//   token = first index whose running sum of p exceeds (u20 * sum(p)) >> 20     (exact_llm.py:243-259);
+//           the last index where none does
 #include <cooperative_groups.h>
 
 #include "exb_internal.h"
@@ -266,7 +267,7 @@ __global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(con
   __syncthreads();
   const uint32_t total = gps[0], before = gps[1];
   const uint32_t target = (uint32_t)(((uint64_t)u * total) >> 20);
-  if (total == 0) {                                           // a row whose every p rounds to 0
+  if (target >= total) {                                      // every p rounds to 0, or u20 is 2^20 or more
     if (c == 0 && tid == 0) a.sampled[r] = a.V - 1;
   } else if (before <= target && target < before + lps) {     // one CTA: its segment, then its lane
     // every warp looks for the segment, a lane over NS neighbouring ones; the segment's own warp goes on

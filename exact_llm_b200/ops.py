@@ -39,7 +39,8 @@ token at a time).  The arithmetic is the exact program's, so a tree gives the bi
                                               (``tree_masks`` makes it from the parents)
     exp_t int32 (10242)                       the Q24 table (``tables.exp_table``)
     logits int64 (R, V), tnum                 rows as the head gives them, round(2^16 / temperature)
-    u20 int32 (R)                             the random number of every row, -1 for the argmax
+    u20 int32 (R)                             the random number of every row, below 2^20 (from there on the
+                                              row's token is V - 1); -1 for the argmax
     tokens, parent int32 (R)                  drafted token and parent node (before its child; root -1)
     status int32 (1)                          gets bit 8 or-ed in where an index was out of range; the
                                               entry is left out, never read or written

@@ -128,7 +128,8 @@ int exb_tree_attention(const exb_kv_view* kv, const int16_t* q, const int32_t* q
 /* Verification of drafted trees against the target's own choice (exact_llm.py:243-259).  Row r's
  * logits (int64, row stride ld) give sampled[r]: the first index whose running sum of the Q20
  * probabilities of shr(logit * tnum, 16) exceeds (u20[r] * total) >> 20, or, where u20[r] < 0, the
- * lowest index of the largest logit.  Then, for every sequence, the walk from node 0: at node c the
+ * lowest index of the largest logit.  u20 is below 2^20; from there on no sum exceeds the target, and
+ * sampled[r] is V - 1.  Then, for every sequence, the walk from node 0: at node c the
  * target's token is sampled[c]; the lowest node whose parent is c and whose token equals it is
  * accepted and the walk goes on there, otherwise it ends.
  *   tokens, parent int32 (R): the drafted token of every row and its parent's index in the sequence

@@ -47,6 +47,25 @@ def test_attention_lowest_32_bit_score(gpu, exp_t, wide, below):  # noqa: F811
 
 # ------------------------------------------------------------------------------------------ verification
 @pytest.mark.gpu
+@pytest.mark.parametrize("V,tnum", [(1, 1 << 16), (97, 1 << 16), (5000, 81920), (152064, 1 << 16), (300000, 1 << 16),
+                                    (400001, 1 << 16), (97, 1 << 32)])
+def test_verify_numbers_past_the_range(gpu, exp_t, V, tnum):  # noqa: F811
+    """u20 from 2^20 on: the last index, on every path."""
+    torch = gpu
+    p = _verify_problem(V, V, [6], greedy=0.0, tnum=tnum)
+    p["u20"][:] = [1 << 20, 2**31 - 1, (1 << 20) - 1, (1 << 20) + 1, 0, 1 << 30]
+    inside = dict(p, u20=np.where(p["u20"] < 1 << 20, p["u20"], 0))
+    want = ref.verify(**inside)[0]
+    want[p["u20"] >= 1 << 20] = V - 1
+    p["tokens"][:] = V                                       # nothing agrees
+    junk = [torch.full((n,), -77, dtype=torch.int32, device="cuda") for n in (1, 6, 6, 6, 6)]
+    del junk
+    sampled, n, path, tok = _verify(torch, exp_t, p)
+    assert np.array_equal(sampled, want)
+    assert n.tolist() == [1] and path[0, 0] == 0 and tok[0, 0] == V - 1
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V", [262143, 262144, 262145, 327680])
 def test_verify_flat_rows(gpu, exp_t, V):  # noqa: F811
     """Equal logits of 2^18 entries and more: sums around 2^42."""
