@@ -342,7 +342,10 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
       }
     }
   }
-  if (!mbar_wait(&tbar, 0)) set_err(a.status, ERR_WAIT_TIMEOUT);             // the table
+  if (!mbar_wait(&tbar, 0)) {                                // the table
+    set_err(a.status, ERR_WAIT_TIMEOUT);
+    mbar_wait(&tbar, 0);                                     // no copy is left in flight
+  }
   __syncthreads();
   // ---- phase 2: e over the stored scores, row sums
 #pragma unroll 1

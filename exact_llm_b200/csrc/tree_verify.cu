@@ -173,7 +173,9 @@ __global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(con
   const int any_big = __syncthreads_or(big != 0);
   if (warp == 0) {
     m = __reduce_max_sync(0xffffffffu, red[lane & (NW - 1)]);
-    if (lane == 0) { lmax = m; lwide = any_big; }
+    // where the table did not come within the wait's limit, the row goes to sample_row, which reads it in place
+    const bool late = u >= 0 && !mbar_wait(&tbar, 0);
+    if (lane == 0) { lmax = m; lwide = any_big || late; }
   }
   cluster.sync();
   // one warp reads the peers' words, all at once, and leaves the result to the CTA: a word of another
@@ -188,8 +190,8 @@ __global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(con
   const int M = gmax;
   const bool wide = gwide;
   if (wide) {
-    if (u >= 0 && !mbar_wait(&tbar, 0)) return;               // no copy is left in flight
     if (c == 0) sample_row<TV_THREADS>(a, r);
+    if (u >= 0) mbar_wait(&tbar, 0);                          // no copy is left in flight
     cluster.sync();
     return;
   }
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(TV_THREADS, IT > 10 ? 2 : 3) k_tree_sample(con
     cluster.sync();
     return;
   }
-  mbar_wait(&tbar, 0);
+  mbar_wait(&tbar, 0);                                        // (complete: warp 0 has seen it; every thread reads the copy)
   uint32_t es = 0;                                            // at most 2^24 each, 40 a thread
 #pragma unroll
   for (int k = 0; k < 2 * IT; ++k) {
