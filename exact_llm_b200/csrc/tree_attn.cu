@@ -51,6 +51,22 @@ struct TreeGeo {
 // score row pitch for n positions: 4 mod 16 words, so a warp's stores and loads hit 32 banks
 inline int tree_pitch(int64_t n) { return (int)((n + 15) / 16 * 16 + 4); }
 
+// zeros in the rows that no sequence owns, the gaps between the ranges taken (see TreeOrder): `n` values of a row
+static __device__ __noinline__ void zero_rows(const int32_t* row_start, const int32_t* ctx, int B, int R, int64_t* out, int pitch, int n) {
+  int end = 0, top = INT32_MIN;
+  for (int b = 0; b <= B; ++b) {
+    const int lo = b < B ? row_start[b] : R, hi = b < B ? row_start[b + 1] : R;
+    const bool taken = lo >= max(top, 0) && hi >= lo && hi <= R && (b == B || (hi > lo && ctx[b] >= 0));
+    if (b < B) top = max(top, lo);
+    if (!taken && b < B) continue;
+    for (int64_t e = threadIdx.x; e < (int64_t)(lo - end) * n; e += TC_THREADS_T) {
+      const int64_t r = e / n;
+      out[(end + r) * pitch + (e - r * n)] = 0;
+    }
+    end = hi;
+  }
+}
+
 template <int HD, int NT>
 __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(const TreeArgs a, int ldk, bool same) {
   using G = TreeGeo<HD, NT>;
@@ -81,13 +97,15 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
   if (warp == 0) {
     int at = 0, fb = -1, ft = 0;
     bool odd = lane == 0 && (a.B == 0 || a.row_start[0] != 0 || a.row_start[a.B] != a.R);
+    TreeOrder order;
     for (int b0 = 0; b0 < a.B && (fb < 0 || blockIdx.x == 0); b0 += 32) {
       const int b = b0 + lane;
       TreeSeq s;
       if (b < a.B) {
         s = tree_seq(a, b, blockIdx.x == 0 && j == 0);
-        odd |= s.T != a.row_start[b + 1] - a.row_start[b];
+        odd |= s.T != s.hi - s.lo;
       }
+      tree_in_order(b < a.B, lane, s, order);
       const int nt = (s.T * a.rep + NR - 1) / NR;
       int inc = nt;
 #pragma unroll
@@ -108,18 +126,7 @@ __global__ void __launch_bounds__(TC_THREADS_T, NT == 1 ? 2 : 1) k_tree_cluster(
     }
   }
   __syncthreads();
-  // rows that no sequence owns: zeros, from the first CTA of every KV head
-  if (blockIdx.x == 0 && odd_sh) {
-    for (int r = warp; r < a.R; r += 8) {
-      bool own = false;
-      for (int b = lane; b < a.B; b += 32) {
-        const TreeSeq s = tree_seq(a, b, false);
-        own |= r >= s.r0 && r < s.r0 + s.T;
-      }
-      if (!__any_sync(0xffffffffu, own))
-        for (int e = lane; e < a.rep * HD; e += 32) a.out[((size_t)r * a.H + j * a.rep) * HD + e] = 0;
-    }
-  }
+  if (blockIdx.x == 0 && odd_sh) zero_rows(a.row_start, a.ctx, a.B, a.R, a.out + j * a.rep * HD, a.H * HD, a.rep * HD);
   const int b = find[0];
   if (b < 0) return;                                         // the whole cluster leaves together
   const TreeSeq sq = tree_seq(a, b, false);

@@ -136,10 +136,12 @@ __global__ void __launch_bounds__(256) k_tt_init(const TreeArgs a, const TtWork 
   if (blockIdx.x == 0 && threadIdx.x < 32) {
     const int lane = threadIdx.x;
     int64_t at0 = 0, at1 = 0;
+    TreeOrder order;
     if (lane == 0) w.pre[0] = w.pre[a.B + 1] = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
       TreeSeq s;
       if (b0 + lane < a.B) s = tree_seq(a, b0 + lane, true);
+      tree_in_order(b0 + lane < a.B, lane, s, order);
       const int64_t rows = (int64_t)s.T * a.rep, nk = (s.S + TT_BK - 1) / TT_BK;
       int64_t u0 = (rows + TtGeo<0>::NR - 1) / TtGeo<0>::NR * nk * a.kv.KV;
       int64_t u1 = (rows + TtGeo<2>::NR - 1) / TtGeo<2>::NR * nk * a.kv.KV;

@@ -42,11 +42,14 @@ struct TreeSeq {
   int r0 = 0, T = 0;                     // first row, nodes
   int ctx = 0;                           // positions that every row sees
   int S = 0;                             // ctx + nodes that have a position in the table
+  int lo = 0, hi = 0;                    // row_start as it is
 };
 
 EXB_DEV TreeSeq tree_seq(const TreeArgs& a, int b, bool report) {
   TreeSeq s;
   const int lo = a.row_start[b], hi = a.row_start[b + 1], c = a.ctx[b];
+  s.lo = lo;
+  s.hi = hi;
   bool bad = lo < 0 || hi > a.R || hi < lo || c < 0;
   if (!bad) {
     s.r0 = lo;
@@ -57,6 +60,32 @@ EXB_DEV TreeSeq tree_seq(const TreeArgs& a, int b, bool report) {
   }
   if (bad && report) set_err(a.status, ERR_BOUNDS);
   return s;
+}
+
+// A warp over all sequences in order, 32 at a time: where row_start falls (tree_seq has reported it), ranges may
+// overlap, and one that begins below an earlier entry is left out too.  So no row belongs to two sequences.
+struct TreeOrder {
+  bool fell = false;
+  int top = 0;                           // the largest entry so far, once it fell
+};
+// (m: this lane's entry, or the lowest number; returns the largest entry up to it)
+static __device__ __noinline__ int tree_top(int m) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 1; i < 32; i <<= 1) {
+    const int w = __shfl_up_sync(0xffffffffu, m, i);
+    if (lane >= i) m = max(m, w);
+  }
+  return m;
+}
+EXB_DEV void tree_in_order(bool there, int lane, TreeSeq& s, TreeOrder& o) {
+  if (!__any_sync(0xffffffffu, s.hi < s.lo) && !o.fell) return;
+  int m = there ? s.lo : INT32_MIN;
+  if (o.fell && lane == 0) m = max(m, o.top);                // (where it rose so far, nothing is above this entry)
+  m = tree_top(m);
+  if (there && s.lo < m) s.T = s.S = 0;
+  o.fell = true;
+  o.top = __shfl_sync(0xffffffffu, m, 31);
 }
 
 // page of position pos, or -1 (reported) where the table names none

@@ -114,6 +114,8 @@ typedef struct exb_kv_view {
  * Sequence b owns rows row_start[b] .. row_start[b+1]-1 of q (its tree, node i = row row_start[b]+i,
  * cached at position ctx[b] + i).  A row sees the positions below ctx[b] and the nodes i whose bit
  * i % 64 of mask[row][i / 64] is set; a row that sees nothing gives zeros.
+ * row_start rises; a range that falls, leaves 0..R or begins below an earlier entry is left out (rows of
+ * no sequence are zeros).
  *   q int16 (R, H, hd), qs int32 (R, H) shifts (0..63); layer 0 of kv is used; H % KV == 0
  *   table int32 (B, max_pages), ctx int32 (B), row_start int32 (B+1), mask (R, mask_words)
  *   exp_t int32 (10242) the program's Q24 table (entry 0 is 2^24); out int64 (R, H, hd)

@@ -45,6 +45,57 @@ def test_attention_lowest_32_bit_score(gpu, exp_t, wide, below):  # noqa: F811
     assert np.array_equal(_attend(gpu, exp_t, p, None, wide).cpu().numpy(), want)
 
 
+@pytest.mark.gpu
+@WIDE
+@pytest.mark.parametrize("hd,nodes", [(16, 3), (128, 100)])
+def test_attention_overlapping_rows(gpu, exp_t, wide, hd, nodes):  # noqa: F811
+    """Where row_start falls, the range that falls and the ones that begin before an earlier one's end are left out:
+    their rows are zeros, and the others have their values."""
+    torch = gpu
+    p = ref.problem(13, H=14, KV=2, hd=hd, page=64, ctx=[70, 20, 30, 9], nodes=[2 * nodes, 0, nodes, 5], words=8)
+    a, b, R = 2 * nodes, 3 * nodes, 3 * nodes + 5
+    want = ref.attention(**p)
+    want[a:b] = 0
+    bad = dict(p, row_start=np.array([0, a, nodes, b, R], np.int32))       # 1: falls; 2: begins inside 0's rows
+    table = np.full((4, 64), -1, np.int32)
+    table[:, :p["table"].shape[1]] = p["table"]
+    table[2, :] = 0                                          # (all of its positions would be there)
+    bad["table"] = table
+    for _ in range(2):
+        junk = torch.full((R, 14, hd), -1, dtype=torch.int64, device="cuda")
+        del junk                                             # what the output's memory holds before the call
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        got = _attend(torch, exp_t, bad, status, wide).cpu().numpy()
+        assert int(status) == 8
+        assert np.array_equal(got, want)
+
+
+@pytest.mark.gpu
+@WIDE
+@pytest.mark.parametrize("falls", [(4,), (31,), (32,), (33, 34), (5, 32, 64), (69,)])
+def test_attention_overlapping_rows_of_many(gpu, exp_t, wide, falls):  # noqa: F811
+    """The same among 70 sequences: the two ranges around an entry that is too low are out, no other."""
+    torch = gpu
+    rng = np.random.default_rng(14)
+    nodes, ctx = rng.integers(1, 7, 70), rng.integers(0, 50, 70)
+    p = ref.problem(14, H=8, KV=2, hd=32, page=16, ctx=[int(x) for x in ctx], nodes=[int(x) for x in nodes])
+    want = ref.attention(**p)
+    rs = p["row_start"].copy()
+    for i in falls:
+        rs[i] = max(rs[i] - 9, 0)
+    for b in range(70):
+        if rs[b] < rs[:b + 1].max() or rs[b + 1] < rs[b]:
+            want[p["row_start"][b]:p["row_start"][b + 1]] = 0
+        else:                                                # the others are as they were
+            assert (rs[b], rs[b + 1]) == (p["row_start"][b], p["row_start"][b + 1])
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    junk = torch.full(want.shape, -1, dtype=torch.int64, device="cuda")
+    del junk
+    got = _attend(torch, exp_t, dict(p, row_start=rs), status, wide).cpu().numpy()
+    assert int(status) == 8
+    assert np.array_equal(got, want)
+
+
 # ------------------------------------------------------------------------------------------ verification
 @pytest.mark.gpu
 @pytest.mark.parametrize("V,tnum", [(1, 1 << 16), (97, 1 << 16), (5000, 81920), (152064, 1 << 16), (300000, 1 << 16),
