@@ -116,7 +116,7 @@ EXB_DEV int k_shift(const exb_kv_view& kv, int head, int pg, int off) {
 //   sum >= 2^42: p is at most 4, the number of j in 1..4 with e >= t_j = ceil(j * sum / 2^20).  inv is the largest
 //     ceil(j * 2^66 / t_j): no smaller one takes t_j to j, and t_j - 1 stays below j, since 2^86 / sum lies between
 //     all j * 2^66 / t_j and all j * 2^66 / (t_j - 1), and two such fractions that differ are 2^18 apart or more
-EXB_DEV uint64_t prob_inverse_long(uint64_t sum) {
+static __device__ __noinline__ uint64_t prob_inverse_long(uint64_t sum) {
   uint64_t inv = 0;
 #pragma unroll 1
   for (uint64_t j = 1; j <= 4; ++j) {
