@@ -44,7 +44,7 @@ constexpr int TT_BK = 128;                         // positions per unit
 constexpr int TT_CHUNK = 32;                       // a chunk is 32 to 63 units of positions (all, if fewer): its row
                                                    // tiles follow one another, so its cache rows are read from L2
                                                    // by all but the first; a run is a part of a chunk
-constexpr uint32_t TT_WAIT_LIMIT = 1u << 20;       // polls of a wait (a limit that depends on earlier waits costs 4%)
+constexpr uint32_t TT_WAIT_LIMIT = 1u << 20;       // polls of a wait
 constexpr int TT_RING = 8;                         // units whose rows' places are kept
 
 struct TtPlaces {                                  // where a unit's cache rows lie, in elements, and the shifts
@@ -227,10 +227,13 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
   //   bar_q   a run's query digits are in place, and what the last run left in shared memory is used up
   //           (two by turns as well: a warp that issues scores has no part in a run of one tile, but in the next)
   //   ring_full, ring_free   a unit's places are written, every warp is done with them
-  __shared__ uint64_t bar_s[2], bar_f[2], bar_k[2], bar_kf[2], bar_v[2], bar_w[2], bar_p, bar_q[2], ring_full[TT_RING], ring_free[TT_RING];
+  //   bar_x   an issuing warp's MMAs are all complete
+  __shared__ uint64_t bar_s[2], bar_f[2], bar_k[2], bar_kf[2], bar_v[2], bar_w[2], bar_p, bar_q[2], ring_full[TT_RING], ring_free[TT_RING], bar_x[3];
   __shared__ uint32_t tmem_sh;
   __shared__ int qmax_sh;
   __shared__ volatile uint32_t top_sh[2];                    // the last unit (+ 1) with a third digit in some p
+  __shared__ volatile uint32_t late_sh;                      // a wait has given up: every role leaves at its next unit
+  __shared__ uint32_t stop_sh;                               // the same, as the softmax warps agree on it at a run's start
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const exb_kv_view& kv = a.kv;
 
@@ -249,7 +252,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
       mbar_init(&ring_free[i], TT_CW + TT_LW);
     }
     mbar_init(&bar_p, 2);                                    // two warps issue the products
-    top_sh[0] = top_sh[1] = 0;
+    for (int i = 0; i < 3; ++i) mbar_init(&bar_x[i], 1);
+    top_sh[0] = top_sh[1] = late_sh = 0;
     mbar_fence_init();
   }
   if (warp == TT_CW + TT_LW) {
@@ -270,11 +274,17 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
   const int64_t total = pre[a.B];
   int64_t u = total * blockIdx.x / gridDim.x;
   const int64_t uend = total * (blockIdx.x + 1) / gridDim.x;
-  bool late = false;                                         // a wait gave up
+  bool gave_up = false;                                      // a wait of this thread
   uint32_t tiles = 0, units = 0, runs = 0;                   // of this CTA so far
-  // the n-th completion (from 0) of a barrier; once a wait has given up, none waits any more and the kernel ends
+  // the n-th completion (from 0) of a barrier.  Where a wait gives up, every warp ends the unit it is in (a few
+  // waits, each with its limit) and the kernel leaves with a status.  The flag is looked at once a unit: 828 us
+  // against 806 without (61 nodes after 32768 tokens); a branch at every wait took 1033
   auto wait = [&](uint64_t* bar, uint32_t n) {
-    late |= !mbar_wait(bar, n & 1, TT_WAIT_LIMIT);
+    gave_up |= !mbar_wait(bar, n & 1, TT_WAIT_LIMIT);
+  };
+  auto late = [&]() {                                        // asked by a warp once a unit
+    if (gave_up) late_sh = 1;
+    return (bool)__any_sync(0xffffffffu, late_sh);
   };
   auto wait2 = [&](uint64_t* bar, uint32_t n) { wait(bar + (n & 1), n >> 1); };          // one of two, by turns
   auto arrive = [&](uint64_t* bar) {                         // this warp, after all its lanes
@@ -310,7 +320,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
         return true;
       };
       bool more = next_pages();
-      while (more) {
+      while (more && !late()) {
         const uint32_t slot = units % TT_RING;
         TtPlaces& out = ring[slot];
         int64_t k[4], v[4];
@@ -362,14 +372,14 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
       using C1 = std::integral_constant<int, 1>;
       using C2 = std::integral_constant<int, 2>;
       using C3 = std::integral_constant<int, 3>;
-      while (u < uend) {
+      while (u < uend && !late_sh) {
         const TtRun run = tt_run(a, pre, G::NR, u, uend);
         u += run.nk;
         if constexpr (PASS < 2) {
           bool begun = false;
           const TreeSeq sq = tree_seq(a, run.b, false);
           const int nh = sq.T * a.rep - run.rt * G::NR > NT ? 2 : 1;
-          for (int i = 0; i < run.nk; ++i, ++units) {
+          for (int i = 0; i < run.nk && !late_sh; ++i, ++units) {
             for (int h = 0; h < nh; ++h, ++tiles) {
               const int s = tiles & 1;
               if (role != s) continue;
@@ -386,7 +396,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
           }
         } else if (role == 0) {
           wait2(bar_q, runs);
-          for (int i = 0; i < run.nk; ++i, ++units) {
+          for (int i = 0; i < run.nk && !late_sh; ++i, ++units) {
             wait2(bar_k, units);
             if (i > 0) wait(&bar_f[0], units - 1);
             tc_fence_after();
@@ -395,7 +405,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
             tc_commit(&bar_kf[units & 1]);
           }
         } else if (role < 3) {
-          for (int i = 0; i < run.nk; ++i, ++units) {
+          for (int i = 0; i < run.nk && !late_sh; ++i, ++units) {
             wait2(bar_v, units);
             wait2(bar_w, units);
             tc_fence_after();
@@ -425,6 +435,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
         }
         ++runs;
       }
+      tc_commit(&bar_x[role]);                               // none is left in flight, however this warp got here
+      mbar_wait(&bar_x[role], 0, TT_WAIT_LIMIT);
     }
     __syncwarp();
   } else if (warp >= TT_CW) {
@@ -483,16 +495,16 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
     };
     const uint32_t all = (uint32_t)(uend - u);
     if constexpr (PASS < 2) {
-      for (; units < all; ++units) {
+      for (; units < all && !late(); ++units) {
         keys(units);
         arrive(&ring_free[units % TT_RING]);
       }
     } else {
       if (all) keys(0);
-      while (u < uend) {
+      while (u < uend && !late()) {
         const TtRun run = tt_run(a, pre, G::NR, u, uend);
         u += run.nk;
-        for (int i = 0; i < run.nk; ++i, ++units) {
+        for (int i = 0; i < run.nk && !late(); ++i, ++units) {
           if (units + 1 < all) keys(units + 1);              // a unit ahead of V, which waits for the products
           const TtPlaces& p = ring[units % TT_RING];
           int4 x[VB * 4];
@@ -524,14 +536,19 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
       u += nk;
       const int g0 = run.rt * G::NR, ng = min(G::NR, sq.T * a.rep - g0);
       const int nh = PASS < 2 && ng > NT ? 2 : 1;
+      if (gave_up) late_sh = 1;
       named_sync(1, TT_COMPUTE);                             // the last run is done with shared memory
-      if (tid == 0) qmax_sh = 0;
+      if (tid == 0) {
+        qmax_sh = 0;
+        stop_sh = late_sh;
+      }
       if (tid < G::NR && tid < ng) {                         // row i of the tile: node (g0 + i) / rep
         const int node = (g0 + tid) / a.rep;
         rowq[tid] = (int64_t)(sq.r0 + node) * a.H + (int64_t)run.j * a.rep + (g0 + tid - node * a.rep);
         rmask[tid] = a.mask + (size_t)(sq.r0 + node) * a.W;
       }
       named_sync(1, TT_COMPUTE);
+      if (stop_sh) break;                                    // all of them or none
       for (int e = tid; e < nh * NT * KCH; e += TT_COMPUTE) {          // query digits
         const int r = e / KCH, c = e - r * KCH;
         int4 v = make_int4(0, 0, 0, 0);
@@ -612,7 +629,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
 #pragma unroll
           for (int r = 0; r < RPT; ++r) { mx[h][r] = INT32_MIN; es[h][r] = 0; }
 #pragma unroll 1
-        for (int i = 0; i < nk; ++i, ++units) {
+        for (int i = 0; i < nk && !late(); ++i, ++units) {
           await_places(units);
           const int ksh = ring[units % TT_RING].s[key];      // shift of this thread's key; -1: no such position
           const int t = (kt0 + i) * TT_BK + key;
@@ -739,7 +756,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
         const uint32_t p0 = sb + G::OFF_P + cg * 128 + (((key >> 4) ^ cg) << 4) + (key & 15);
         const uint32_t p1 = sb + G::OFF_P + cg * 128 + (((key >> 4) ^ (4 + cg)) << 4) + (key & 15);
 #pragma unroll 1
-        for (int i = 0; i < nk; ++i, ++units) {
+        for (int i = 0; i < nk && !late(); ++i, ++units) {
           await_places(units);
           const int ksh = ring[units % TT_RING].s[key];      // shift of this thread's key; -1: no such position
           const int t = (kt0 + i) * TT_BK + key;
@@ -834,8 +851,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_tt(const TreeArgs a, const Tt
       }
     }
   }
-  if (late) set_err(a.status, ERR_WAIT_TIMEOUT);
+  if (gave_up) late_sh = 1;
   __syncthreads();
+  if (tid == 0 && late_sh) set_err(a.status, ERR_WAIT_TIMEOUT);
   if (warp == TT_CW + TT_LW)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
