@@ -394,12 +394,12 @@ class ExactModel:
             raise ValueError("tree_step: as many parents as ids")
         start = np.concatenate([[0], np.cumsum([len(t[1]) for t in trees])]).astype(np.int32)
         B, R = len(trees), int(start[-1])
-        ml = int(max_len or max((len(t[1]) for t in trees), default=1))
+        ml = max((len(t[1]) for t in trees), default=1) if max_len is None else int(max_len)
         u = None if u20 is None else np.ascontiguousarray(np.asarray(u20, np.int32).reshape(-1))
         if u is not None and len(u) != R:
             raise ValueError("tree_step: one random number per node")
         seqs = np.asarray(slots, np.int32)
-        n, path, toks = np.empty(B, np.int32), np.empty((B, ml), np.int32), np.empty((B, ml), np.int32)
+        n, path, toks = np.empty(B, np.int32), *(np.empty((B, max(ml, 0)), np.int32) for _ in range(2))
         logits = np.empty((R, self.c["V"]), np.int64) if want_logits else None
         self._rows = R
         check(lib.exb_tree_step(self.h, B, ptr(seqs, ctypes.c_int32), ptr(start, ctypes.c_int32),

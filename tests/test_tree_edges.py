@@ -144,3 +144,15 @@ def test_tree_step_row_ranges(cuda_ok, starts):
     rc = lib.exb_tree_step(m.h, B, seqs, rs, ids, par, None, 1 << 16, 4, n, path, tok, None, None)
     assert rc == 1 and "row_start must rise" in lib.exb_last_error().decode()
     assert [lib.exb_seq_len(m.h, s) for s in range(3)] == [3, 3, 3]
+
+
+@pytest.mark.gpu
+def test_tree_step_no_length(cuda_ok):
+    """A max_len of 0 or less is refused by the engine, not taken for the default."""
+    from exact_llm_b200 import ExbError
+    from tests.test_tree_decode import SMALL, _model, _prompt
+    m = _model(SMALL, max_batch=1, max_seq=40)
+    m.forward(_prompt(SMALL, 10), m.new_cache(0))
+    for n in (0, -1):
+        with pytest.raises(ExbError, match="max_len"):
+            m.tree_step([(0, [1, 2], [-1, 0])], max_len=n)
