@@ -45,7 +45,8 @@ token at a time).  The arithmetic is the exact program's, so a tree gives the bi
     status int32 (1)                          gets bit 8 or-ed in where an index was out of range; the
                                               entry is left out, never read or written
 
-They run on the current stream of the tensors' device, never synchronise and can be captured.
+They run on the current stream of the tensors' device, never synchronise and can be captured.  They are in
+libexactb200_torch.so; where it was not built, or for another torch, each of them raises ImportError when called.
 """
 import ctypes
 import os
@@ -89,13 +90,33 @@ def _gemv_fake(x16, wT, Mg):
 
 # ------------------------------------------------------------------------------------------ drafted trees
 # Schemas, checks and calls are in torch_ops.cpp, which gets the entry points of the library loaded by _lib.
-if not os.path.exists(TORCH_OPS_PATH):
-    raise ImportError(f"{TORCH_OPS_PATH} is missing: build it with `python exact_llm_b200/build.py`")
-torch.ops.load_library(TORCH_OPS_PATH)
 _ENTRIES = ("exb_last_error", "exb_tree_attention_workspace_bytes", "exb_tree_attention", "exb_tree_verify",
             "exb_kv_compact", "exb_kv_copy_pages")
-ctypes.CDLL(TORCH_OPS_PATH).exb_torch_bind(
-    (ctypes.c_void_p * len(_ENTRIES))(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p) for n in _ENTRIES)))
+_TREE_OPS = ("tree_attention", "tree_verify", "kv_compact_", "kv_copy_pages_")
+
+
+def _missing(name, why):
+    def op(*args, **kwargs):
+        raise ImportError(f"torch.ops.exact.{name}: {why}; build it with `python exact_llm_b200/build.py`")
+    return op
+
+
+def _load_tree_ops(path):
+    """Register the operators of ``path``.  Without it ``exact::gemv`` is all there is, and the others raise when called."""
+    why = f"{path} is missing"
+    if os.path.exists(path):
+        try:
+            torch.ops.load_library(path)
+            bind = ctypes.CDLL(path).exb_torch_bind
+            bind((ctypes.c_void_p * len(_ENTRIES))(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p) for n in _ENTRIES)))
+            return
+        except (OSError, AttributeError) as e:               # of another torch, or older than this module
+            why = f"{path} does not load ({e})"
+    for name in _TREE_OPS:
+        setattr(torch.ops.exact, name, _missing(name, why))
+
+
+_load_tree_ops(TORCH_OPS_PATH)
 
 
 def tree_masks(parent, row_start, words=None):
