@@ -87,8 +87,12 @@ def build_torch(force=False, verbose=False):
         print("torch is not installed: no torch operators")
         return None
     newest = max(os.path.getmtime(p) for p in (TORCH_SRC, os.path.join(ROOT, "include", "exactb200.h")))
-    if not force and os.path.exists(TORCH_LIB) and os.path.getmtime(TORCH_LIB) > newest:
-        return TORCH_LIB
+    made_for = f"{torch.__version__} {os.path.dirname(torch.__file__)}"       # the library fits this torch alone
+    stamp = os.path.join(OBJ, "torch_ops.torch")
+    if not force and os.path.exists(TORCH_LIB) and os.path.getmtime(TORCH_LIB) > newest and os.path.exists(stamp):
+        with open(stamp) as f:
+            if f.read() == made_for:
+                return TORCH_LIB
     import sysconfig
     cuda = os.path.dirname(os.path.dirname(NVCC))
     inc = include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda, "include"), os.path.join(ROOT, "include")]
@@ -103,6 +107,9 @@ def build_torch(force=False, verbose=False):
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+    os.makedirs(OBJ, exist_ok=True)
+    with open(stamp, "w") as f:
+        f.write(made_for)
     return TORCH_LIB
 
 

@@ -1,4 +1,5 @@
-"""The operator module without the library of the drafted-tree operators."""
+"""The operator module without the library of the drafted-tree operators, and when that library is built anew."""
+import importlib.util
 import os
 import subprocess
 import sys
@@ -45,3 +46,25 @@ def test_ops_without_the_torch_library(tmp_path, there):
     r = subprocess.run([sys.executable, str(tmp_path / "use.py")], cwd=tmp_path, capture_output=True, text=True,
                        env=dict(os.environ, PYTHONPATH=str(tmp_path)), timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_torch_library_is_built_anew_for_another_torch(tmp_path, monkeypatch):
+    torch = pytest.importorskip("torch")
+    spec = importlib.util.spec_from_file_location("exb_build_copy", os.path.join(ROOT, "exact_llm_b200", "build.py"))
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    calls = []
+
+    def compiler(cmd, **kw):
+        calls.append(cmd)
+        with open(cmd[cmd.index("-o") + 1], "w") as f:
+            f.write("library")
+
+    monkeypatch.setattr(b, "TORCH_LIB", str(tmp_path / "lib.so"))
+    monkeypatch.setattr(b, "OBJ", str(tmp_path / "obj"))
+    monkeypatch.setattr(b.subprocess, "run", compiler)
+    for version, builds in (("9.1", 1), ("9.1", 1), ("9.2", 2), ("9.2", 2), ("9.1", 3)):
+        monkeypatch.setattr(torch, "__version__", version)
+        assert b.build_torch() == str(tmp_path / "lib.so") and len(calls) == builds, version
+    b.build_torch(force=True)
+    assert len(calls) == 4
