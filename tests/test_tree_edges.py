@@ -156,3 +156,91 @@ def test_tree_step_no_length(cuda_ok):
     for n in (0, -1):
         with pytest.raises(ExbError, match="max_len"):
             m.tree_step([(0, [1, 2], [-1, 0])], max_len=n)
+
+
+def _check_step(m, p, ids, par, nodes, layers):
+    """One step of slot 0 (which holds p) on a tree: the logits of `nodes`, the tokens and the cache are those of plain
+    steps along the paths (slot 1, forked from slot 0)."""
+    from exact_llm_b200 import Cache
+    ((path, toks),), lg = m.tree_step([(0, ids, par)], want_logits=True)
+
+    def way(i):
+        out = []
+        while i >= 0:
+            out.append(ids[i])
+            i = par[i]
+        return np.array(out[::-1], np.int32)
+
+    for i in nodes:
+        c = m.fork(0, 1, len(p))
+        assert np.array_equal(m.forward(way(i), c, last_only=True)[-1], lg[i]), i
+    assert path[0] == 0 and all(par[b] == a and ids[b] == t for a, b, t in zip(path, path[1:], toks))
+    assert toks == [int(np.argmax(lg[i])) for i in path]
+    assert not any(par[i] == path[-1] and ids[i] == toks[-1] for i in range(len(ids)))
+    m.forward(way(path[-1]), m.fork(0, 1, len(p)))
+    for i in range(layers):
+        a, b = m.kv_cache(i, Cache(m, 0)), m.kv_cache(i, Cache(m, 1))
+        assert a["kq"].shape[1] == len(p) + len(path)
+        assert all(np.array_equal(a[n], b[n]) for n in ("kq", "sk", "v"))
+    return path
+
+
+def _tree(rng, V, chain, n):
+    """`chain` from the root on, and random nodes around it."""
+    ids, par, on = [int(chain[0])], [-1], 0
+    for i in range(1, n):
+        if i % 3 == 1 and i // 3 + 1 < len(chain):
+            ids.append(int(chain[i // 3 + 1]))
+            par.append(on)
+            on = i
+        else:
+            ids.append(int(rng.integers(0, V)))
+            par.append(int(rng.integers(max(0, i - 70), i)))
+    return ids, par
+
+
+@pytest.mark.gpu
+def test_tree_step_long_context(cuda_ok):
+    """One layer of the 7B architecture, 4500 tokens in a cache of 8192 and a tree of 70 nodes: the attention's tcgen05
+    kernels, and masks of two words."""
+    from exact_llm_b200 import configs
+    from tests.test_tree_decode import _model, _prompt
+    c = configs.arch("qwen2.5-7b", NL=1)
+    m = _model(c, max_batch=2, max_seq=8192)
+    p = _prompt(c, 4500, 6)
+    m.forward(p, m.new_cache(0), want_logits=False)
+    first = int(m.last_next[-1])
+    cache, chain = m.fork(0, 1), [first]
+    for _ in range(5):                                       # what plain steps give
+        m.forward(np.array(chain[-1:], np.int32), cache, want_logits=False)
+        chain.append(int(m.last_next[-1]))
+    ids, par = _tree(np.random.default_rng(6), c["V"], chain, 70)
+    assert len(_check_step(m, p, ids, par, [0, 1, 4, 7, 33, 63, 64, 69], 1)) >= 5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("moe,rows", [(False, 512), (True, 256)], ids=["dense", "moe"])
+def test_tree_step_most_rows(cuda_ok, moe, rows):
+    """As many nodes as a step takes, in one tree and in two; one more is refused."""
+    from exact_llm_b200 import ExbError
+    from tests.test_tree_decode import MOE, SMALL, _model, _prompt
+    c = MOE if moe else SMALL
+    rng = np.random.default_rng(rows)
+    m = _model(c, max_batch=3, max_seq=900)
+    p = _prompt(c, 50, 7)
+    m.forward(p, m.new_cache(0))
+    chain = [int(m.last_next[-1])]
+    cache = m.fork(0, 1)
+    for _ in range(9):
+        m.forward(np.array(chain[-1:], np.int32), cache)
+        chain.append(int(m.last_next[-1]))
+    ids, par = _tree(rng, c["V"], chain, rows + 1)
+    with pytest.raises(ExbError, match="rows"):
+        m.tree_step([(0, ids, par)])
+    keep = m.fork(0, 2)
+    assert len(_check_step(m, p, ids[:-1], par[:-1], [0, 1, 63, 64, 200, rows - 1], c["NL"])) >= 9
+    a, b = rows // 3, rows - rows // 3                       # slots 2 and 1, of the same prompt
+    m.fork(2, 0), m.fork(2, 1)
+    (one,), lg1 = m.tree_step([(0, ids[:a], par[:a])], want_logits=True)
+    both, lg = m.tree_step([(1, ids[:b], par[:b]), (keep, ids[:a], par[:a])], want_logits=True)
+    assert both[1] == one and np.array_equal(lg[b:], lg1)
