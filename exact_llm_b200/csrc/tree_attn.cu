@@ -7,11 +7,12 @@
 // gives the same bits), so a row goes over its scores three times.  Here the scores stay in shared memory
 // meanwhile; tree_tc.cu computes them anew each time, for many rows and long caches.
 //
-// Measured on one B200 (device time in a graph): 32 single tokens of 28 heads after up to 1000 tokens 28.5 us
+// Measured on one B200 (device time in a graph): 32 single tokens of 28 heads after up to 1000 tokens 28.8 us
 // (11.4 us would be the 75 MB at the rate of a copy; every SM reads rows of 256 and 512 bytes by look-up, and
-// what it has in flight covers the latency of L2 and HBM in part); a tree of 26 nodes of 28 heads after 513
-// tokens 21.7 us and one token of an empty sequence 9.6 us (cluster barriers and the chain from the lengths
-// over the table to the rows: no bytes to speak of).
+// what it has in flight covers the latency of L2 and HBM in part: 126 registers a thread and the shared memory
+// each leave room for two CTAs); a tree of 26 nodes of 28 heads after 513 tokens 21.9 us and one token of an
+// empty sequence 9.4 us (cluster barriers and the chain from the lengths over the table to the rows: no bytes to
+// speak of).  Width 16 with 8 rows a tile spills one register (4 bytes stored, 8 loaded), no other does.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -520,7 +521,11 @@ static cudaError_t launch_cluster_hd(const TreeArgs& a, int C, int ldk, bool sam
 }
 
 // The tensor-core kernels from about 7 million scores of 128 dims on, with rows enough in a group to fill
-// their tiles.  Measured both ways (28 heads of 128, 4 groups; one tree of 16, 32, 64 nodes): after 2000
+// their tiles.  The lengths are on the device, so the rule takes a.cap, what a table row has room for: the figures
+// are of tables as wide as the cache is long.  In wider ones the choice, the cluster size and the shared memory are
+// those of the longer cache (a tree of 26 nodes of 28 heads after 513 tokens in tables of 1024, 4096, 16384
+// positions 22, 33, 62 us; 32 single tokens after 1000 in 1024, 4096, 16384, 32768, 131072: 29, 40, 111, 218, 97).
+// Measured both ways (28 heads of 128, 4 groups; one tree of 16, 32, 64 nodes): after 2000
 // tokens 28, 43, 83 us here and 61, 72, 97 there; after 8000 tokens 68, 129, 254 here and 91, 120, 179
 // there; 8 trees of 16 nodes of 40 heads, 8 groups, after 1000, 2000, 4000 tokens 78, 147, 239 and 99, 145,
 // 212; at half the width it takes twice the scores (64 nodes of 14 heads after 8000, 16000 tokens: 90, 176

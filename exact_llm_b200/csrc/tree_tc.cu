@@ -19,12 +19,13 @@
 // Scores are computed anew in each kernel: keeping them would move 12 bytes a score, more than the MMAs
 // and the three multiply-adds that make one cost.
 //
-// Measured on one B200 (device time in a graph): a tree of 61 nodes of 40 heads after 32768 tokens 791 us,
-// 24 digit products of 128 dims a score, 0.62 POP/s; 8 trees of up to 63 nodes of 28 heads after up to 4097
-// tokens 476 us.  A unit of the third kernel takes about 9000 cycles: 17 thousand warp instructions (the
-// exact exp table with its interpolation, the division by the sum, byte digits) at 2.1 a cycle, and of the
-// shared memory's cycles 4400 for their loads and stores (1900 are conflicts of the table's random look-ups)
-// and 2800 for the MMAs' operands; the tensor cores are busy a sixth of the time.
+// Measured on one B200 (device time in a graph): a tree of 61 nodes of 40 heads after 32768 tokens 817 us,
+// 24 digit products of 128 dims a score, 0.60 POP/s; 8 trees of up to 63 nodes of 28 heads after up to 4097
+// tokens 491 us.  Every kernel spills (width 128, bytes stored and loaded: 40 and 132, 52 and 148, 68 and 296):
+// 72 registers are all that 896 threads can start with.  A unit of the third kernel takes about 9000 cycles: 17
+// thousand warp instructions (the exact exp table with its interpolation, the division by the sum, byte digits) at
+// 2.0 a cycle, and of the shared memory's cycles 4400 for their loads and stores (1900 are conflicts of the table's
+// random look-ups) and 2800 for the MMAs' operands; the tensor cores are busy a sixth of the time.
 #include <algorithm>
 #include <type_traits>
 
@@ -99,7 +100,7 @@ EXB_DEV void sts8(uint32_t a, uint32_t x) {
   asm volatile("{\n .reg .b16 t;\n cvt.u16.u32 t, %1;\n st.shared.u8 [%0], t;\n}\n" ::"r"(a), "r"(x) : "memory");
 }
 // one MMA with its descriptors put together inside: low words base + constant, the common high word.  Few
-// registers live across a row of them (the MMA warp has 32; a spilled operand is a trip to L2)
+// registers live across a row of them (the MMA warp has 48; a spilled operand is a trip to L2)
 constexpr uint32_t TT_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);    // as tc_desc
 template <int DOFF, int AOFF, int BOFF, uint32_t IDESC>
 EXB_DEV void tt_mma(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {

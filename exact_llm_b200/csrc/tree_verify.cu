@@ -90,9 +90,9 @@ __global__ void __launch_bounds__(1024) k_tree_sample_long(const VerArgs a) { sa
 // thread and step), so the row is read once while the cluster agrees on its maximum and its sum.  What
 // stays is the scaled logit as 32 bits, then e, then p; the sum of all p is at most 2^20, so 32-bit sums
 // do from there.  A row with a scaled logit of 2^30 or more goes to sample_row instead.
-// Measured on one B200 (device time in a graph): 420 rows of 152064 logits 257 us, 2.0 TB/s (a copy moves
+// Measured on one B200 (device time in a graph): 420 rows of 152064 logits 259 us, 2.0 TB/s (a copy moves
 // 6.6: the loads, the look-ups in the exp table and three agreements of the cluster follow one another within a
-// row, and two or three CTAs an SM cover one another's only in part); 26 rows 21 us, one greedy row 8 us with
+// row, and two or three CTAs an SM cover one another's only in part); 26 rows 22 us, one greedy row 8 us with
 // the walk.
 constexpr int TV_THREADS = 512;
 
